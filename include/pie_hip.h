@@ -36,8 +36,9 @@ enum {
 const char* pie_hip_last_error(void);
 
 /* ABI version; bumped whenever a declaration below changes or is added (2: paged attention and
- * sampling; 3: attention sinks; 4: cut prefill plans, sliced sampling and softmax). */
-#define PIE_HIP_ABI_VERSION 4
+ * sampling; 3: attention sinks; 4: cut prefill plans, sliced sampling and softmax; 5: first tokens kept
+ * beside a window, log-sum-exps, shared prefixes, joined states). */
+#define PIE_HIP_ABI_VERSION 5
 int pie_hip_abi_version(void); /* of the library: PIE_HIP_ABI_VERSION where header and library match */
 
 /*
@@ -462,6 +463,108 @@ int pie_hip_attention_prefill_split(const pie_bf16* q, int64_t q_tok_stride, int
                                     pie_bf16* out, int64_t o_tok_stride, int64_t o_head_stride,
                                     void* stream);
 
+/*
+ * The decode and prefill forms with two additions (all other arguments as above).
+ * first_tokens: the request's first tokens that stay visible beside the window: the query at position p
+ * sees t <= p (mode 1; mode 0: any t; mode 2: mask bits) with t >= p - window_left or t < first_tokens.
+ * Without a window (window_left < 0) it has no effect. Pages that hold hidden positions only are not read,
+ * but for the page-table entries of a window's first 31 positions before it.
+ * lse: NULL, or fp32 [tokens, num_qo_heads] contiguous: log2 of the row's softmax mass,
+ * log2 sum_t 2^(q . k_t * sm_scale * log2 e); -inf for a row that sees nothing. Not with sinks.
+ * pie_hip_attention_decode_lse's workspace is pie_hip_attention_decode's. pie_hip_attention_prefill_first_plan
+ * is pie_hip_attention_prefill_split_plan for a run at these first_tokens; a run of it at another mode,
+ * window_left or first_tokens takes its uncut items. split: the plan's (NULL: an uncut plan).
+ */
+int pie_hip_attention_decode_lse(const pie_bf16* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                 const pie_bf16* k_cache, const pie_bf16* v_cache, int64_t page_stride,
+                                 int64_t slot_stride, int64_t head_stride, int64_t num_pages,
+                                 const int32_t* kv_indptr, const int32_t* kv_indices,
+                                 const int32_t* kv_last_page_len, int64_t batch, int64_t num_qo_heads,
+                                 int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                 float sm_scale, int64_t window_left, int64_t first_tokens,
+                                 const float* sinks, int64_t splits, void* workspace,
+                                 int64_t workspace_bytes, pie_bf16* out, int64_t o_tok_stride,
+                                 int64_t o_head_stride, float* lse, void* stream);
+int pie_hip_attention_prefill_first_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                         const int32_t* kv_last_page_len, int64_t batch,
+                                         int64_t page_size, int64_t num_qo_heads,
+                                         int64_t num_kv_heads, int64_t head_dim, int32_t mode,
+                                         int64_t window_left, int64_t first_tokens, int64_t num_cus,
+                                         int64_t workspace_bytes, int32_t* plan,
+                                         int64_t plan_capacity, int64_t* plan_words,
+                                         int64_t* num_items, int64_t* mask_bytes,
+                                         int64_t* mask_words, int64_t* split);
+int pie_hip_attention_prefill_lse(const pie_bf16* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                  const pie_bf16* k_cache, const pie_bf16* v_cache,
+                                  int64_t page_stride, int64_t slot_stride, int64_t head_stride,
+                                  int64_t num_pages, const int32_t* qo_indptr,
+                                  const int32_t* kv_indptr, const int32_t* kv_indices,
+                                  const int32_t* kv_last_page_len, int64_t num_qo_heads,
+                                  int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                  float sm_scale, int32_t mode, int64_t window_left,
+                                  int64_t first_tokens, const float* sinks,
+                                  const uint32_t* packed_mask, const int32_t* mask_extent,
+                                  const int32_t* plan, int64_t num_items, int64_t mask_offsets_word,
+                                  const int64_t* split, void* scratch, int64_t scratch_bytes,
+                                  pie_bf16* out, int64_t o_tok_stride, int64_t o_head_stride,
+                                  float* lse, void* stream);
+
+/*
+ * Attention of a batch whose requests share prefixes that the cache holds once: forked contexts, beams,
+ * many requests behind one system prompt. Requests come in groups: group g holds requests
+ * group_indptr[g] .. group_indptr[g+1] - 1 and its prefix is the run of pages
+ * prefix_indices[prefix_indptr[g] .. prefix_indptr[g+1]), the last holding prefix_last_page_len[g]
+ * tokens; each request's own tokens (its suffix) are its pages in kv_indptr / kv_indices /
+ * kv_last_page_len. A query token sees its group's whole prefix and, of its request's suffix, every
+ * token (one query token per request, qo_indptr NULL) or those up to itself (qo_indptr: the request's
+ * query tokens are its suffix's last ones). Prefixes and suffixes may be empty; a row that sees nothing is
+ * 0. Cache addressing, heads, scale and lse as in the decode and prefill forms; one query token per
+ * request needs num_qo_heads / num_kv_heads <= 16.
+ *
+ * pie_hip_attention_shared_plan runs on the host over host tables and writes the work list (`plan`, int32
+ * words that the caller copies to the device; NULL: only info is filled, info[0] = its words) and
+ * info[16] for the run (info[1] = the scratch bytes it needs, at most scratch_bytes). num_cus: the
+ * device's compute units (0: 256). The run reads prefix_indices and the suffix tables on the device: with
+ * one query token per request one plan, and one captured run, serve suffixes of any length (the lengths
+ * at plan time only steer how the work is cut); with qo_indptr the plan holds for its own lengths.
+ * scratch (16-byte aligned) holds partial results from the run's first launch to its second: runs that
+ * share it must not overlap. One made while another stream's run uses it, or between another thread's
+ * launches, returns PIE_HIP_EBUSY; runs recorded under graph capture are not checked.
+ * No counterpart in the reference, whose wrappers read a shared prefix once per request; it serves the
+ * calls at pie/src/pie_worker/model/llama3.py:765-790, :689.
+ */
+int pie_hip_attention_shared_plan(const int32_t* group_indptr, int64_t groups,
+                                  const int32_t* prefix_indptr, const int32_t* prefix_last_page_len,
+                                  const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                  const int32_t* kv_last_page_len, int64_t batch, int64_t page_size,
+                                  int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
+                                  int64_t num_cus, int64_t scratch_bytes, int32_t* plan,
+                                  int64_t plan_capacity, int64_t* info);
+int pie_hip_attention_shared(const pie_bf16* q, int64_t q_tok_stride, int64_t q_head_stride,
+                             const pie_bf16* k_cache, const pie_bf16* v_cache, int64_t page_stride,
+                             int64_t slot_stride, int64_t head_stride, int64_t num_pages,
+                             const int32_t* prefix_indices, const int32_t* kv_indptr,
+                             const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                             int64_t num_tokens, int64_t num_qo_heads, int64_t num_kv_heads,
+                             int64_t head_dim, int64_t page_size, float sm_scale, const int32_t* plan,
+                             const int64_t* info, void* scratch, int64_t scratch_bytes, pie_bf16* out,
+                             int64_t o_tok_stride, int64_t o_head_stride, float* lse, void* stream);
+
+/*
+ * The join of attention results over disjoint parts of a context: part i of row (t, h) holds its
+ * normalised output (parts, bf16 or fp32) and log2 softmax mass (lses, fp32);
+ *   M = max_i l_i,  out = sum_i 2^(l_i - M) o_i / sum_i 2^(l_i - M),  lse = M + log2 sum_i 2^(l_i - M).
+ * Parts with l_i = -inf count for nothing, whatever they hold; a row without any other is 0 with lse
+ * -inf. Statistics and sums are fp32; out has the parts' type. head_dim in {64, 128, 256}; strides in
+ * elements, rows 16-byte aligned. out may be one of the parts, lse one of the lses.
+ */
+int pie_hip_attention_merge_states(const void* parts, int32_t is_bf16, int64_t part_stride,
+                                   int64_t part_tok_stride, int64_t part_head_stride,
+                                   const float* lses, int64_t lse_part_stride,
+                                   int64_t lse_tok_stride, int64_t lse_head_stride, int64_t num_parts,
+                                   int64_t num_tokens, int64_t num_heads, int64_t head_dim, void* out,
+                                   int64_t o_tok_stride, int64_t o_head_stride, float* lse,
+                                   int64_t e_tok_stride, int64_t e_head_stride, void* stream);
 
 /*
  * Sampling from probabilities, one draw per row: flashinfer.sampling.sampling_from_probs (mode 0),

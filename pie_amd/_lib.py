@@ -62,6 +62,19 @@ SIGNATURES: dict[str, list] = {
     "pie_hip_attention_prefill_split": [vp, i64, i64, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, i64,
                                         i64, i64, i64, f32, i32, i64, vp, vp, vp, vp, i64, i64, vp, vp,
                                         i64, vp, i64, i64, vp],
+    "pie_hip_attention_decode_lse": [vp, i64, i64, vp, vp, i64, i64, i64, i64, vp, vp, vp, i64, i64,
+                                     i64, i64, i64, f32, i64, i64, vp, i64, vp, i64, vp, i64, i64, vp, vp],
+    "pie_hip_attention_prefill_first_plan": [vp, vp, vp, i64, i64, i64, i64, i64, i32, i64, i64, i64, i64,
+                                             vp, i64, vp, vp, vp, vp, vp],
+    "pie_hip_attention_prefill_lse": [vp, i64, i64, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, i64,
+                                      i64, i64, i64, f32, i32, i64, i64, vp, vp, vp, vp, i64, i64, vp, vp,
+                                      i64, vp, i64, i64, vp, vp],
+    "pie_hip_attention_shared_plan": [vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, vp,
+                                      i64, vp],
+    "pie_hip_attention_shared": [vp, i64, i64, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, i64, i64, i64,
+                                 i64, i64, f32, vp, vp, vp, i64, vp, i64, i64, vp, vp],
+    "pie_hip_attention_merge_states": [vp, i32, i64, i64, i64, vp, i64, i64, i64, i64, i64, i64, i64, vp,
+                                       i64, i64, vp, i64, i64, vp],
     "pie_hip_sample": [vp, i64, i64, i64, i64, vp, i32, vp, i32, vp, f32, vp, f32, vp, u64, u64, vp, vp],
     "pie_hip_sample_workspace": [i64, i64, i32],
     "pie_hip_sample_sliced": [vp, i64, i64, i64, i64, vp, i32, vp, i32, vp, f32, vp, f32, vp, u64, u64, vp,
@@ -77,7 +90,7 @@ SIGNATURES: dict[str, list] = {
     "pie_hip_get_batch_indices_positions": [vp, vp, i64, i64, vp, vp, vp],
 }
 RETURNS_I64 = {"pie_hip_sample_workspace", "pie_hip_scaled_softmax_workspace"}
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _lib: C.CDLL | None = None
 

@@ -12,13 +12,20 @@ The API is flashinfer 0.6.1's, restated in pie/src/flashinfer_metal/ops.py:163-2
                                          whose softmax denominators hold a per-head sink logit
                                          -> pie_hip_attention_decode (one query token per
                                          request) or pie_hip_attention_prefill
+    BatchSharedPrefixAttentionWrapper    groups of requests behind prefixes that the cache holds
+                                         once -> pie_hip_attention_shared
+    merge_attention_states               the join of results over disjoint parts of a context
+                                         -> pie_hip_attention_merge_states
 
-``plan`` runs on the host and allocates nothing on the device; ``run`` launches kernels on the
-current stream and allocates only its output (unless ``out=`` is given), so it can be captured.
-Split requests keep their partial results in the caller's workspace buffer, as flashinfer does.
-``window_left`` (flashinfer's sliding window, which OLMo-3 plans per layer) is supported; the
-options Pie's models do not use (positional encodings inside attention, logit soft caps, lse
-output, fp8 scales) raise instead of being ignored.
+``plan`` runs on the host and allocates nothing on the device (a shared-prefix plan: its work list);
+``run`` launches kernels on the current stream and allocates only its output (unless ``out=`` is
+given), so it can be captured. Split requests keep their partial results in the caller's workspace
+buffer, as flashinfer does. ``window_left`` (flashinfer's sliding window, which OLMo-3 plans per layer)
+is supported, and so are first tokens that stay visible beside it (``first_tokens``, this package's
+extension): the query at position p sees t <= p with t >= p - window_left or t < first_tokens.
+``return_lse=True`` also returns each row's log2 of its softmax mass, fp32 [tokens, heads] (-inf for a
+row that sees nothing). The options Pie's models do not use (positional encodings inside attention,
+logit soft caps, fp8 scales) raise instead of being ignored.
 """
 from __future__ import annotations
 
@@ -34,7 +41,8 @@ from . import _lib
 from .ops import _cache_desc, _check, _stream
 
 __all__ = ["BatchDecodeWithPagedKVCacheWrapper", "BatchPrefillWithPagedKVCacheWrapper",
-           "BatchAttentionWithAttentionSinkWrapper"]
+           "BatchAttentionWithAttentionSinkWrapper", "BatchSharedPrefixAttentionWrapper",
+           "merge_attention_states"]
 
 _BF16 = torch.bfloat16
 _CUS: dict = {}
@@ -53,6 +61,29 @@ def _unsupported(name: str, pos_encoding_mode="NONE", logits_soft_cap=None):
                                   "applied before the append, as Pie does)")
     if logits_soft_cap not in (None, 0, 0.0):
         raise NotImplementedError(f"{name}: logits_soft_cap={logits_soft_cap}")
+
+
+def _not_empty(indices: torch.Tensor) -> torch.Tensor:
+    """A page list with an address: an empty tensor has none, and a batch that holds no page reads none."""
+    return indices if indices.numel() else torch.zeros(1, dtype=torch.int32, device=indices.device)
+
+
+def _first(name: str, first_tokens) -> int:
+    if first_tokens is None:
+        return 0
+    if isinstance(first_tokens, bool) or int(first_tokens) != first_tokens or first_tokens < 0:
+        raise ValueError(f"{name}: first_tokens must be a whole number >= 0, got {first_tokens!r}")
+    return int(first_tokens)
+
+
+def _lse_out(name: str, lse: Optional[torch.Tensor], return_lse: bool, rows: int, heads: int, like: torch.Tensor):
+    """The tensor a call writes its log-sum-exps to: the caller's, a new one, or none."""
+    if lse is None:
+        return torch.empty((rows, heads), dtype=torch.float32, device=like.device) if return_lse else None
+    _check(name, torch.float32, lse=lse)
+    if lse.device != like.device or tuple(lse.shape) != (rows, heads) or not lse.is_contiguous():
+        raise ValueError(f"{name}: lse must be a contiguous [{rows}, {heads}] tensor on {like.device}")
+    return lse
 
 
 class BatchDecodeWithPagedKVCacheWrapper:
@@ -86,10 +117,11 @@ class BatchDecodeWithPagedKVCacheWrapper:
              logits_soft_cap: Optional[float] = None, q_data_type=torch.float16,
              kv_data_type=None, data_type=None, sm_scale: Optional[float] = None,
              rope_scale: Optional[float] = None, rope_theta: Optional[float] = None,
-             non_blocking: bool = True, **_ignored) -> None:
+             non_blocking: bool = True, first_tokens: int = 0, **_ignored) -> None:
         name = "BatchDecodeWithPagedKVCacheWrapper.plan"
         _unsupported(name, pos_encoding_mode, logits_soft_cap)
         window_left = -1 if window_left is None or window_left < 0 else int(window_left)
+        first = _first(name, first_tokens) if window_left >= 0 else 0
         if num_kv_heads <= 0 or num_qo_heads % num_kv_heads:
             raise ValueError(f"{name}: num_qo_heads {num_qo_heads} is not a multiple of "
                              f"num_kv_heads {num_kv_heads}")
@@ -110,6 +142,9 @@ class BatchDecodeWithPagedKVCacheWrapper:
             np_ = (indptr[1:] - indptr[:-1]).to(torch.int64)
             if batch:
                 max_kv = int(((np_ - 1).clamp(min=0) * page_size + last_page_len.to(torch.int64)).max())
+        if first:  # no request shows more than its window and the first tokens
+            shown = min(window_left + 1 + first, 2**31)
+            max_kv = shown if max_kv < 0 else min(max_kv, shown)
         splits = C.c_int64(0)
         dev = self._workspace.device
         cus = _num_cus(dev) if dev.type == "cuda" else 0
@@ -125,9 +160,10 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if any(t.device.type != "cuda" for t in (indptr, indices, last_page_len)):
             indptr, indices, last_page_len = (t.to(dev, non_blocking=non_blocking)
                                               for t in (indptr, indices, last_page_len))
+        indices = _not_empty(indices)
         self._plan = dict(indptr=indptr, indices=indices, last_page_len=last_page_len,
                           batch=batch, Hq=num_qo_heads, Hkv=num_kv_heads, D=head_dim,
-                          P=page_size, splits=s, window_left=window_left,
+                          P=page_size, splits=s, window_left=window_left, first=first,
                           sm_scale=(1.0 / math.sqrt(head_dim)) if sm_scale is None else sm_scale)
 
     begin_forward = plan
@@ -141,15 +177,15 @@ class BatchDecodeWithPagedKVCacheWrapper:
         p = self._plan
         if p is None:
             raise RuntimeError(f"{name}: plan() must be called before run()")
-        if return_lse or lse is not None:
-            raise NotImplementedError(f"{name}: lse output")
+        if (return_lse or lse is not None) and _sinks is not None:
+            raise NotImplementedError(f"{name}: lse output with sinks")
         if q_scale not in (None, 1.0) or k_scale not in (None, 1.0) or v_scale not in (None, 1.0):
             raise NotImplementedError(f"{name}: quantisation scales")
         if _lib.fast is not None:
             r = _lib.fast.attention_decode(p, q, paged_kv_cache, self._kv_layout, self._workspace, out,
-                                           _sinks)
+                                           _sinks, lse if lse is not None else return_lse)
             if r is not None:
-                return r
+                return r if return_lse or lse is None else r[0]
         _check(name, _BF16, q=q)
         _check(name, torch.int32, indptr=p["indptr"], indices=p["indices"],
                last_page_len=p["last_page_len"])
@@ -166,15 +202,18 @@ class BatchDecodeWithPagedKVCacheWrapper:
             _check(name, _BF16, out=out)
             if tuple(out.shape) != (B, Hq, D) or out.stride(2) != 1:
                 raise ValueError(f"{name}: out must be [{B}, {Hq}, {D}]")
+        e = _lse_out(name, lse, return_lse, B, Hq, q)
         ws = self._workspace
-        _lib.call("pie_hip_attention_decode", q.data_ptr(), q.stride(0), q.stride(1), kp, vp, ps,
+        more = p["first"] > 0 or e is not None
+        _lib.call("pie_hip_attention_decode_lse" if more else "pie_hip_attention_decode", q.data_ptr(), q.stride(0), q.stride(1), kp, vp, ps,
                   ss, hs, npages, p["indptr"].data_ptr(), p["indices"].data_ptr(),
                   p["last_page_len"].data_ptr(), B, Hq, Hkv, D, P, float(p["sm_scale"]),
-                  p["window_left"], None if _sinks is None else _sinks.data_ptr(), p["splits"],
+                  p["window_left"], *((p["first"],) if more else ()),
+                  None if _sinks is None else _sinks.data_ptr(), p["splits"],
                   ws.data_ptr(), ws.numel() * ws.element_size(),
                   out.data_ptr(),
-                  out.stride(0), out.stride(1), _stream(q))
-        return out
+                  out.stride(0), out.stride(1), *((None if e is None else e.data_ptr(),) if more else ()), _stream(q))
+        return (out, e) if return_lse else out
 
     forward = run
 
@@ -208,10 +247,11 @@ class BatchPrefillWithPagedKVCacheWrapper:
              sm_scale: Optional[float] = None, window_left: int = -1,
              logits_soft_cap: Optional[float] = None, rope_scale: Optional[float] = None,
              rope_theta: Optional[float] = None, q_data_type=torch.float16, kv_data_type=None,
-             non_blocking: bool = True, **_ignored) -> None:
+             non_blocking: bool = True, first_tokens: int = 0, **_ignored) -> None:
         name = "BatchPrefillWithPagedKVCacheWrapper.plan"
         _unsupported(name, pos_encoding_mode, logits_soft_cap)
         window_left = -1 if window_left is None or window_left < 0 else int(window_left)
+        first = _first(name, first_tokens) if window_left >= 0 else 0
         if head_dim_vo not in (None, head_dim_qk):
             raise NotImplementedError(f"{name}: head_dim_vo {head_dim_vo} != head_dim_qk")
         if num_kv_heads <= 0 or num_qo_heads % num_kv_heads:
@@ -243,8 +283,8 @@ class BatchPrefillWithPagedKVCacheWrapper:
         plan = np.empty(cap, dtype=np.int32)
         words, items, mbytes, mwords = C.c_int64(0), C.c_int64(0), C.c_int64(0), C.c_int64(0)
         split = (C.c_int64 * 7)()
-        _lib.call("pie_hip_attention_prefill_split_plan", qo_h.data_ptr(), kv_h.data_ptr(), ll_h.data_ptr(),
-                  batch, page_size, num_qo_heads, num_kv_heads, head_dim_qk, mode, window_left, cus, ws_bytes,
+        _lib.call("pie_hip_attention_prefill_first_plan", qo_h.data_ptr(), kv_h.data_ptr(), ll_h.data_ptr(),
+                  batch, page_size, num_qo_heads, num_kv_heads, head_dim_qk, mode, window_left, first, cus, ws_bytes,
                   plan.ctypes.data, cap, C.byref(words), C.byref(items), C.byref(mbytes), C.byref(mwords), split)
         if mode == 2:
             if mask.dtype not in (torch.bool, torch.uint8):
@@ -271,6 +311,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         plan_d.copy_(torch.from_numpy(plan[: words.value]), non_blocking=False)
         tables = [t if t.device == dev else t.to(dev) for t in
                   (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)]
+        tables[2] = _not_empty(tables[2])
         packed = extent = None
         if mode == 2 and mwords.value:
             packed = ws8[mask_off: mask_off + mwords.value * 4].view(torch.int32)
@@ -282,7 +323,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         self._plan = dict(qo_indptr=tables[0], indptr=tables[1], indices=tables[2],
                           last_page_len=tables[3], batch=batch, T=T, Hq=num_qo_heads,
                           Hkv=num_kv_heads, D=head_dim_qk, P=page_size, mode=mode, packed=packed, extent=extent,
-                          window_left=window_left,
+                          window_left=window_left, first=first,
                           plan=plan_d, items=items.value, woff_word=int(plan[4]), split=split,
                           scratch=ws8[scratch_off: scratch_off + split[4]],
                           sm_scale=(1.0 / math.sqrt(head_dim_qk)) if sm_scale is None else sm_scale)
@@ -298,15 +339,15 @@ class BatchPrefillWithPagedKVCacheWrapper:
         p = self._plan
         if p is None:
             raise RuntimeError(f"{name}: plan() must be called before run()")
-        if return_lse or lse is not None:
-            raise NotImplementedError(f"{name}: lse output")
+        if (return_lse or lse is not None) and _sinks is not None:
+            raise NotImplementedError(f"{name}: lse output with sinks")
         if q_scale not in (None, 1.0) or k_scale not in (None, 1.0) or v_scale not in (None, 1.0):
             raise NotImplementedError(f"{name}: quantisation scales")
         if _lib.fast is not None:
             r = _lib.fast.attention_prefill(p, q, paged_kv_cache, self._kv_layout, C.addressof(p["split"]),
-                                            out, _sinks)
+                                            out, _sinks, lse if lse is not None else return_lse)
             if r is not None:
-                return r
+                return r if return_lse or lse is None else r[0]
         _check(name, _BF16, q=q)
         _check(name, torch.int32, qo_indptr=p["qo_indptr"], indptr=p["indptr"],
                indices=p["indices"], last_page_len=p["last_page_len"])
@@ -323,20 +364,26 @@ class BatchPrefillWithPagedKVCacheWrapper:
             _check(name, _BF16, out=out)
             if tuple(out.shape) != (T, Hq, D) or out.stride(2) != 1:
                 raise ValueError(f"{name}: out must be [{T}, {Hq}, {D}]")
+        e = _lse_out(name, lse, return_lse, T, Hq, q)
         packed = p["packed"]
         if p["mode"] == 2 and packed is None:  # a mask over zero positions: nothing is visible
-            return out.zero_()
+            out.zero_()
+            if e is not None:
+                e.fill_(-math.inf)
+            return (out, e) if return_lse else out
         scratch = p["scratch"]
-        _lib.call("pie_hip_attention_prefill_split", q.data_ptr(), q.stride(0), q.stride(1), kp, vp, ps,
+        more = p["first"] > 0 or e is not None
+        _lib.call("pie_hip_attention_prefill_lse" if more else "pie_hip_attention_prefill_split", q.data_ptr(), q.stride(0), q.stride(1), kp, vp, ps,
                   ss, hs, npages, p["qo_indptr"].data_ptr(), p["indptr"].data_ptr(),
                   p["indices"].data_ptr(), p["last_page_len"].data_ptr(), Hq, Hkv, D, P,
-                  float(p["sm_scale"]), p["mode"], p["window_left"],
+                  float(p["sm_scale"]), p["mode"], p["window_left"], *((p["first"],) if more else ()),
                   None if _sinks is None else _sinks.data_ptr(),
                   packed.data_ptr() if packed is not None else None,
                   p["extent"].data_ptr() if p["extent"] is not None else None,
                   p["plan"].data_ptr(), p["items"], p["woff_word"], p["split"], scratch.data_ptr(),
-                  scratch.numel(), out.data_ptr(), out.stride(0), out.stride(1), _stream(q))
-        return out
+                  scratch.numel(), out.data_ptr(), out.stride(0), out.stride(1),
+                  *((None if e is None else e.data_ptr(),) if more else ()), _stream(q))
+        return (out, e) if return_lse else out
 
     forward = run
 
@@ -372,7 +419,7 @@ class BatchAttentionWithAttentionSinkWrapper:
              num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
              causal: bool = True, window_left: Optional[int] = None, sm_scale: Optional[float] = None,
              q_data_type=torch.bfloat16, kv_data_type=None, non_blocking: bool = True,
-             **_ignored) -> None:
+             first_tokens: int = 0, **_ignored) -> None:
         name = "BatchAttentionWithAttentionSinkWrapper.plan"
         if not causal:
             raise NotImplementedError(f"{name}: causal=False")
@@ -383,12 +430,13 @@ class BatchAttentionWithAttentionSinkWrapper:
         if single:
             self._decode.plan(paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len,
                               num_qo_heads, num_kv_heads, head_dim, page_size, window_left=wl,
-                              sm_scale=sm_scale, non_blocking=non_blocking)
+                              sm_scale=sm_scale, non_blocking=non_blocking, first_tokens=first_tokens)
             self._use = self._decode
         else:
             self._prefill.plan(qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len,
                                num_qo_heads, num_kv_heads, head_dim, page_size, causal=True,
-                               window_left=wl, sm_scale=sm_scale, non_blocking=non_blocking)
+                               window_left=wl, sm_scale=sm_scale, non_blocking=non_blocking,
+                               first_tokens=first_tokens)
             self._use = self._prefill
 
     begin_forward = plan
@@ -396,8 +444,11 @@ class BatchAttentionWithAttentionSinkWrapper:
     def run(self, q: torch.Tensor,
             paged_kv_cache: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]],
             sinks: torch.Tensor, sm_scale: Optional[float] = None,
-            out: Optional[torch.Tensor] = None, **_ignored) -> torch.Tensor:
+            out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+            return_lse: bool = False, **_ignored) -> torch.Tensor:
         name = "BatchAttentionWithAttentionSinkWrapper.run"
+        if return_lse or lse is not None:
+            raise NotImplementedError(f"{name}: lse output with sinks")
         if self._use is None:
             raise RuntimeError(f"{name}: plan() must be called before run()")
         if not isinstance(sinks, torch.Tensor) or tuple(sinks.shape) != (self._Hq,):
@@ -418,3 +469,161 @@ class BatchAttentionWithAttentionSinkWrapper:
 
     def end_forward(self) -> None:
         pass
+
+
+class BatchSharedPrefixAttentionWrapper:
+    """Attention of a batch whose requests share prefixes that the cache holds once: forked contexts,
+    beams, many requests behind one system prompt. Pie's wrappers read such a prefix once per request
+    (llama3.py:765-790 plan, :689 run); here the query tokens of a group read theirs together.
+
+    Requests come in groups: group g holds requests group_indptr[g] .. group_indptr[g+1] - 1, its
+    prefix is the pages prefix_indices[prefix_indptr[g] .. prefix_indptr[g+1]), the last of them
+    holding prefix_last_page_len[g] tokens. Each request's own tokens (its suffix) are its pages in the
+    kv tables, as for the other wrappers; a step's new tokens are appended to the suffix. A query token
+    sees its group's whole prefix and its request's suffix: all of it with one query token per request
+    (qo_indptr=None), up to itself where the request's query tokens are the suffix's last
+    qo_indptr[b+1] - qo_indptr[b]. Prefixes and suffixes may be empty.
+
+    ``plan`` reads the index arrays on the host (a copy, for GPU tensors). With one query token per
+    request the suffix tables are read on the device by each run: one plan, and one captured run, serve
+    suffixes of any length, whose lengths at plan time only steer how the work is cut. With qo_indptr a
+    plan holds for its own lengths. Partial results live in the workspace from a run's first launch to
+    its second: give wrappers whose runs overlap in time their own (an eager run while another stream's
+    run uses the workspace raises). A captured run keeps the plan it was captured with."""
+
+    def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
+        if kv_layout not in ("NHD", "HND"):
+            raise ValueError(f"kv_layout must be 'NHD' or 'HND', got {kv_layout!r}")
+        self._workspace = float_workspace_buffer
+        self._kv_layout = kv_layout
+        self._plan = None
+        self._captured = []  # plans that captured graphs read
+
+    def plan(self, group_indptr: torch.Tensor, prefix_indptr: torch.Tensor, prefix_indices: torch.Tensor,
+             prefix_last_page_len: torch.Tensor, paged_kv_indptr: torch.Tensor, paged_kv_indices: torch.Tensor,
+             paged_kv_last_page_len: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_dim: int,
+             page_size: int, qo_indptr: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None) -> None:
+        name = "BatchSharedPrefixAttentionWrapper.plan"
+        groups, batch = group_indptr.numel() - 1, paged_kv_indptr.numel() - 1
+        sizes = {"group_indptr": (group_indptr, groups + 1), "prefix_indptr": (prefix_indptr, groups + 1),
+                 "prefix_last_page_len": (prefix_last_page_len, groups), "paged_kv_indptr": (paged_kv_indptr, batch + 1),
+                 "paged_kv_last_page_len": (paged_kv_last_page_len, batch)}
+        if qo_indptr is not None:
+            sizes["qo_indptr"] = (qo_indptr, batch + 1)
+        if groups < 0 or batch < 0:
+            raise ValueError(f"{name}: empty indptr")
+        host = {}
+        for arg, (t, n) in sizes.items():
+            if t.dim() != 1 or t.numel() != n or t.dtype != torch.int32:
+                raise ValueError(f"{name}: {arg} must be {n} int32 values, got {t.dtype} {tuple(t.shape)}")
+            host[arg] = t.cpu().contiguous()
+        dev = self._workspace.device
+        device = {}
+        for arg, t, n in (("prefix_indices", prefix_indices, int(host["prefix_indptr"][-1])),
+                          ("paged_kv_indices", paged_kv_indices, int(host["paged_kv_indptr"][-1])),
+                          ("paged_kv_indptr", paged_kv_indptr, batch + 1),
+                          ("paged_kv_last_page_len", paged_kv_last_page_len, batch)):
+            if t.dim() != 1 or t.numel() < n or t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError(f"{name}: {arg} must hold at least {n} contiguous int32 values, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+            device[arg] = _not_empty(t.to(dev))
+        ws_bytes = self._workspace.numel() * self._workspace.element_size()
+        scratch_off = -self._workspace.data_ptr() % 16
+        info = (C.c_int64 * 16)()
+        ptr = lambda arg: host[arg].data_ptr() if arg in host else None
+        args = (ptr("group_indptr"), groups, ptr("prefix_indptr"), ptr("prefix_last_page_len"), ptr("qo_indptr"),
+                ptr("paged_kv_indptr"), ptr("paged_kv_last_page_len"), batch, page_size, num_qo_heads, num_kv_heads,
+                head_dim, _num_cus(dev) if dev.type == "cuda" else 0, ws_bytes - scratch_off)
+        _lib.call("pie_hip_attention_shared_plan", *args, None, 0, info)
+        words = np.empty(max(1, info[0]), dtype=np.int32)
+        _lib.call("pie_hip_attention_shared_plan", *args, words.ctypes.data, words.size, info)
+        scratch = self._workspace.view(-1).view(torch.uint8)[scratch_off: scratch_off + info[1]]
+        self._plan = dict(indptr=device["paged_kv_indptr"], indices=device["paged_kv_indices"],
+                          last_page_len=device["paged_kv_last_page_len"], prefix_indices=device["prefix_indices"],
+                          T=info[8], Hq=num_qo_heads, Hkv=num_kv_heads, D=head_dim, P=page_size,
+                          plan=torch.from_numpy(words).to(dev), info=info, info_at=C.addressof(info), scratch=scratch,
+                          sm_scale=(1.0 / math.sqrt(head_dim)) if sm_scale is None else float(sm_scale))
+
+    def run(self, q: torch.Tensor, paged_kv_cache: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]],
+            out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, return_lse: bool = False):
+        """q [tokens, Hq, D] bf16 -> out, and with return_lse (out, lse) as the other wrappers' run."""
+        name = "BatchSharedPrefixAttentionWrapper.run"
+        p = self._plan
+        if p is None:
+            raise RuntimeError(f"{name}: plan() must be called before run()")
+        if p["plan"].is_cuda and torch.cuda.is_current_stream_capturing() and not any(k is p for k in self._captured):
+            self._captured.append(p)
+        if _lib.fast is not None:
+            r = _lib.fast.attention_shared(p, q, paged_kv_cache, self._kv_layout, out, lse if lse is not None else return_lse)
+            if r is not None:
+                return r if return_lse or lse is None else r[0]
+        _check(name, _BF16, q=q)
+        _check(name, torch.int32, plan=p["plan"], paged_kv_indptr=p["indptr"])
+        T, Hq, Hkv, D = p["T"], p["Hq"], p["Hkv"], p["D"]
+        if q.dim() != 3 or tuple(q.shape) != (T, Hq, D) or q.stride(2) != 1:
+            raise ValueError(f"{name}: q must be [{T}, {Hq}, {D}] with unit inner stride, got {tuple(q.shape)}")
+        kp, vp, npages, ps, ss, hs, P = _cache_desc(paged_kv_cache, self._kv_layout, Hkv, D, name)
+        if P != p["P"]:
+            raise ValueError(f"{name}: cache page size {P} != planned {p['P']}")
+        cache0 = paged_kv_cache[0] if isinstance(paged_kv_cache, (tuple, list)) else paged_kv_cache
+        if not q.device == cache0.device == p["plan"].device:
+            raise RuntimeError(f"{name}: q, the cache and the workspace must be on one device")
+        if out is None:
+            out = torch.empty((T, Hq, D), dtype=_BF16, device=q.device)
+        else:
+            _check(name, _BF16, q=q, out=out)
+            if tuple(out.shape) != (T, Hq, D) or out.stride(2) != 1:
+                raise ValueError(f"{name}: out must be [{T}, {Hq}, {D}] with unit inner stride")
+        e = _lse_out(name, lse, return_lse, T, Hq, q)
+        with torch.cuda.device(q.device):
+            _lib.call("pie_hip_attention_shared", q.data_ptr(), q.stride(0), q.stride(1), kp, vp, ps, ss, hs, npages,
+                      p["prefix_indices"].data_ptr(), p["indptr"].data_ptr(), p["indices"].data_ptr(),
+                      p["last_page_len"].data_ptr(), T, Hq, Hkv, D, P, p["sm_scale"], p["plan"].data_ptr(), p["info"],
+                      p["scratch"].data_ptr(), p["scratch"].numel(), out.data_ptr(), out.stride(0), out.stride(1),
+                      None if e is None else e.data_ptr(), _stream(q))
+        return (out, e) if return_lse else out
+
+
+def merge_attention_states(parts: torch.Tensor, lses: torch.Tensor, out: Optional[torch.Tensor] = None,
+                           lse: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Join attention results over disjoint parts of a context: parts [n, tokens, heads, D] (bf16 or
+    float32, D in {64, 128, 256}), each with its log2 softmax mass in lses [n, tokens, heads] (float32,
+    what ``run(..., return_lse=True)`` gives). Returns (out, lse) of the whole context, out in the parts'
+    type: with M = max_i l_i, out = sum_i 2^(l_i - M) o_i / sum_i 2^(l_i - M), lse = M + log2 of that
+    sum. A part with l_i = -inf counts for nothing, whatever it holds; a row without any other is 0 with
+    lse -inf. out may be one of the parts, lse one of the lses."""
+    name = "merge_attention_states"
+    if _lib.fast is not None:
+        r = _lib.fast.merge_states(parts, lses, out, lse)
+        if r is not None:
+            return r
+    if not isinstance(parts, torch.Tensor) or parts.dtype not in (_BF16, torch.float32):
+        raise ValueError(f"{name}: parts must be a bfloat16 or float32 tensor")
+    _check(name, parts.dtype, parts=parts)
+    _check(name, torch.float32, lses=lses)
+    if parts.dim() != 4 or parts.shape[0] < 1 or tuple(lses.shape) != tuple(parts.shape[:3]):
+        raise ValueError(f"{name}: parts must be [n >= 1, tokens, heads, D] and lses [n, tokens, heads], got "
+                         f"{tuple(parts.shape)} and {tuple(lses.shape)}")
+    if lses.device != parts.device:
+        raise RuntimeError(f"{name}: lses is on {lses.device}, expected {parts.device}")
+    S, T, H, D = parts.shape
+    if parts.stride(3) != 1:
+        raise ValueError(f"{name}: parts must have unit inner stride")
+    if out is None:
+        out = torch.empty((T, H, D), dtype=parts.dtype, device=parts.device)
+    else:
+        _check(name, parts.dtype, parts=parts, out=out)
+        if tuple(out.shape) != (T, H, D) or out.stride(2) != 1:
+            raise ValueError(f"{name}: out must be [{T}, {H}, {D}] with unit inner stride")
+    if lse is None:
+        lse = torch.empty((T, H), dtype=torch.float32, device=parts.device)
+    else:
+        _check(name, torch.float32, lses=lses, lse=lse)
+        if tuple(lse.shape) != (T, H):
+            raise ValueError(f"{name}: lse must be [{T}, {H}]")
+    with torch.cuda.device(parts.device):
+        _lib.call("pie_hip_attention_merge_states", parts.data_ptr(), 1 if parts.dtype == _BF16 else 0, parts.stride(0),
+                  parts.stride(1), parts.stride(2), lses.data_ptr(), lses.stride(0), lses.stride(1), lses.stride(2), S,
+                  T, H, D, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0), lse.stride(1),
+                  _stream(parts))
+    return out, lse

@@ -18,6 +18,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -31,7 +32,8 @@ namespace {
   X(pie_hip_abi_version) X(pie_hip_rmsnorm) X(pie_hip_gemma_rmsnorm)                              \
   X(pie_hip_fused_add_rmsnorm) X(pie_hip_gemma_fused_add_rmsnorm) X(pie_hip_silu_and_mul)         \
   X(pie_hip_gelu_tanh_and_mul) X(pie_hip_embedding) X(pie_hip_qk_rmsnorm_rope_append)             \
-  X(pie_hip_attention_decode) X(pie_hip_attention_prefill_split)
+  X(pie_hip_attention_decode) X(pie_hip_attention_prefill_split) X(pie_hip_attention_decode_lse)            \
+  X(pie_hip_attention_prefill_lse) X(pie_hip_attention_shared) X(pie_hip_attention_merge_states)
 struct Lib {
 #define X(name) decltype(&::name) name = nullptr;
   PIE_ENTRY_POINTS(X)
@@ -342,14 +344,45 @@ bool sinks_of(PyObject* o, const at::Device& dev, const float*& p) {
   return true;
 }
 
-// attention_decode(plan, q, cache, kv_layout, workspace, out, sinks)
+// Where log-sum-exps go: the caller's tensor, a new one (True) or nowhere (False).
+struct Lse {
+  at::Tensor t;
+  float* p = nullptr;
+};
+bool lse_of(PyObject* o, const at::Tensor& like, int64_t rows, int64_t heads, Lse& l) {
+  if (o == Py_False) return true;
+  if (o == Py_True) {
+    l.t = at::empty({rows, heads}, at::TensorOptions().dtype(at::kFloat).device(like.device()));
+    if (!l.t.unsafeGetTensorImpl()->has_storage() || l.t.key_set().has_any(kTransforms)) return false;
+  } else {
+    const at::Tensor* t = tensor(o, at::kFloat);
+    if (!t || t->device() != like.device() || t->dim() != 2 || t->size(0) != rows || t->size(1) != heads ||
+        !t->is_contiguous())
+      return false;
+    l.t = *t;
+  }
+  l.p = ptr<float>(l.t);
+  return true;
+}
+// (out, lse), or out alone where no log-sum-exps were asked for.
+PyObject* give_pair(PyObject* out_o, const at::Tensor& out, PyObject* lse_o, const Lse& l) {
+  if (!l.t.defined()) return give(out_o, out);
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, give(out_o, out));
+  PyTuple_SET_ITEM(pair, 1, give(lse_o == Py_True ? Py_None : lse_o, l.t));
+  return pair;
+}
+
+// attention_decode(plan, q, cache, kv_layout, workspace, out, sinks, lse)
 PyObject* attention_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  SERVE(n == 7 && PyDict_CheckExact(a[0]) && !modes_active());
+  SERVE(n == 8 && PyDict_CheckExact(a[0]) && !modes_active());
   const at::Tensor* q = bf16(a[1]);
-  int64_t B, Hq, Hkv, D, P, splits, window;
+  int64_t B, Hq, Hkv, D, P, splits, window, first;
   SERVE(q && whole(a[0], "batch", B) && whole(a[0], "Hq", Hq) && whole(a[0], "Hkv", Hkv) && whole(a[0], "D", D) &&
-        whole(a[0], "P", P) && whole(a[0], "splits", splits) && whole(a[0], "window_left", window));
+        whole(a[0], "P", P) && whole(a[0], "splits", splits) && whole(a[0], "window_left", window) &&
+        whole(a[0], "first", first));
   const auto dev = q->device();
   const at::Tensor *ip = table(a[0], "indptr", dev), *ix = table(a[0], "indices", dev),
                    *ll = table(a[0], "last_page_len", dev);
@@ -368,27 +401,37 @@ PyObject* attention_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   SERVE(sinks_of(a[6], dev, sinks));
   at::Tensor out;
   SERVE(output(a[5], *q, q->sizes(), out) && out.stride(2) == 1);
+  Lse lse;
+  SERVE(lse_of(a[7], *q, B, Hq, lse));
+  const c10::DeviceGuard guard(dev);
   void *st = stream_of(*q), *wp = ws.data_ptr();
   const int64_t wn = ws.numel() * (int64_t)ws.element_size();
   uint16_t *qp = ptr<uint16_t>(*q), *op = ptr<uint16_t>(out);
   const int32_t *ipp = ptr<int32_t>(*ip), *ixp = ptr<int32_t>(*ix), *llp = ptr<int32_t>(*ll);
-  LAUNCH("pie_hip_attention_decode",
-         lib.pie_hip_attention_decode(qp, q->stride(0), q->stride(1), c.k, c.v, c.page, c.slot, c.head, c.pages, ipp,
-                                      ixp, llp, B, Hq, Hkv, D, P, (float)scale, window, sinks, splits, wp, wn, op,
-                                      out.stride(0), out.stride(1), st));
-  return give(a[5], out);
+  if (!first && !lse.p) {
+    LAUNCH("pie_hip_attention_decode",
+           lib.pie_hip_attention_decode(qp, q->stride(0), q->stride(1), c.k, c.v, c.page, c.slot, c.head, c.pages, ipp,
+                                        ixp, llp, B, Hq, Hkv, D, P, (float)scale, window, sinks, splits, wp, wn, op,
+                                        out.stride(0), out.stride(1), st));
+    return give(a[5], out);
+  }
+  LAUNCH("pie_hip_attention_decode_lse",
+         lib.pie_hip_attention_decode_lse(qp, q->stride(0), q->stride(1), c.k, c.v, c.page, c.slot, c.head, c.pages,
+                                          ipp, ixp, llp, B, Hq, Hkv, D, P, (float)scale, window, first, sinks, splits,
+                                          wp, wn, op, out.stride(0), out.stride(1), lse.p, st));
+  return give_pair(a[5], out, a[7], lse);
   END_HANDLE_TH_ERRORS
 }
 
-// attention_prefill(plan, q, cache, kv_layout, split address, out, sinks)
+// attention_prefill(plan, q, cache, kv_layout, split address, out, sinks, lse)
 PyObject* attention_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  SERVE(n == 7 && PyDict_CheckExact(a[0]) && !modes_active());
+  SERVE(n == 8 && PyDict_CheckExact(a[0]) && !modes_active());
   const at::Tensor* q = bf16(a[1]);
-  int64_t T, Hq, Hkv, D, P, mode, window, items, woff;
+  int64_t T, Hq, Hkv, D, P, mode, window, first, items, woff;
   SERVE(q && whole(a[0], "T", T) && whole(a[0], "Hq", Hq) && whole(a[0], "Hkv", Hkv) && whole(a[0], "D", D) &&
         whole(a[0], "P", P) && whole(a[0], "mode", mode) && whole(a[0], "window_left", window) &&
-        whole(a[0], "items", items) && whole(a[0], "woff_word", woff));
+        whole(a[0], "first", first) && whole(a[0], "items", items) && whole(a[0], "woff_word", woff));
   const auto dev = q->device();
   const at::Tensor *qi = table(a[0], "qo_indptr", dev), *ip = table(a[0], "indptr", dev),
                    *ix = table(a[0], "indices", dev), *ll = table(a[0], "last_page_len", dev),
@@ -415,18 +458,106 @@ PyObject* attention_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
   SERVE(sinks_of(a[6], dev, sinks));
   at::Tensor out;
   SERVE(output(a[5], *q, q->sizes(), out) && out.stride(2) == 1);
+  Lse lse;
+  SERVE(lse_of(a[7], *q, T, Hq, lse));
+  const c10::DeviceGuard guard(dev);
   void *st = stream_of(*q), *scp = scratch->data_ptr();
   uint16_t *qp = ptr<uint16_t>(*q), *op = ptr<uint16_t>(out);
   const int32_t *qip = ptr<int32_t>(*qi), *ipp = ptr<int32_t>(*ip), *ixp = ptr<int32_t>(*ix), *llp = ptr<int32_t>(*ll),
                 *plp = ptr<int32_t>(*plan), *exp = extent ? ptr<int32_t>(*extent) : nullptr;
   const uint32_t* pkp = packed ? ptr<uint32_t>(*packed) : nullptr;
   const int64_t scn = scratch->numel();
-  LAUNCH("pie_hip_attention_prefill_split",
-         lib.pie_hip_attention_prefill_split(qp, q->stride(0), q->stride(1), c.k, c.v, c.page, c.slot, c.head, c.pages,
-                                             qip, ipp, ixp, llp, Hq, Hkv, D, P, (float)scale, (int32_t)mode, window,
-                                             sinks, pkp, exp, plp, items, woff, split, scp, scn, op, out.stride(0),
-                                             out.stride(1), st));
-  return give(a[5], out);
+  if (!first && !lse.p) {
+    LAUNCH("pie_hip_attention_prefill_split",
+           lib.pie_hip_attention_prefill_split(qp, q->stride(0), q->stride(1), c.k, c.v, c.page, c.slot, c.head,
+                                               c.pages, qip, ipp, ixp, llp, Hq, Hkv, D, P, (float)scale, (int32_t)mode,
+                                               window, sinks, pkp, exp, plp, items, woff, split, scp, scn, op,
+                                               out.stride(0), out.stride(1), st));
+    return give(a[5], out);
+  }
+  LAUNCH("pie_hip_attention_prefill_lse",
+         lib.pie_hip_attention_prefill_lse(qp, q->stride(0), q->stride(1), c.k, c.v, c.page, c.slot, c.head, c.pages,
+                                           qip, ipp, ixp, llp, Hq, Hkv, D, P, (float)scale, (int32_t)mode, window,
+                                           first, sinks, pkp, exp, plp, items, woff, split, scp, scn, op,
+                                           out.stride(0), out.stride(1), lse.p, st));
+  return give_pair(a[5], out, a[7], lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// attention_shared(plan, q, cache, kv_layout, out, lse)
+PyObject* attention_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  SERVE(n == 6 && PyDict_CheckExact(a[0]) && !modes_active());
+  const at::Tensor* q = bf16(a[1]);
+  int64_t T, Hq, Hkv, D, P, info_at;
+  SERVE(q && whole(a[0], "T", T) && whole(a[0], "Hq", Hq) && whole(a[0], "Hkv", Hkv) && whole(a[0], "D", D) &&
+        whole(a[0], "P", P) && whole(a[0], "info_at", info_at));
+  const auto dev = q->device();
+  const at::Tensor *ip = table(a[0], "indptr", dev), *ix = table(a[0], "indices", dev),
+                   *ll = table(a[0], "last_page_len", dev), *px = table(a[0], "prefix_indices", dev),
+                   *plan = table(a[0], "plan", dev);
+  PyObject *so = field(a[0], "sm_scale"), *sc = field(a[0], "scratch");
+  double scale;
+  SERVE(ip && ix && ll && px && plan && so && sc && f64(so, scale));
+  const at::Tensor* scratch = tensor(sc, at::kByte);
+  SERVE(scratch && scratch->device() == dev);
+  SERVE(q->dim() == 3 && q->size(0) == T && q->size(1) == Hq && q->size(2) == D && q->stride(2) == 1);
+  const int nhd = layout(a[3]);
+  SERVE(nhd >= 0);
+  const Cache c = cache(a[2], nhd == 1, Hkv, D, dev);
+  SERVE(c.ok && c.page_size == P);
+  at::Tensor out;
+  SERVE(output(a[4], *q, q->sizes(), out) && out.stride(2) == 1);
+  Lse lse;
+  SERVE(lse_of(a[5], *q, T, Hq, lse));
+  const c10::DeviceGuard guard(dev);
+  void *st = stream_of(*q), *scp = scratch->data_ptr();
+  uint16_t *qp = ptr<uint16_t>(*q), *op = ptr<uint16_t>(out);
+  const int32_t *ipp = ptr<int32_t>(*ip), *ixp = ptr<int32_t>(*ix), *llp = ptr<int32_t>(*ll), *pxp = ptr<int32_t>(*px),
+                *plp = ptr<int32_t>(*plan);
+  const int64_t *info = reinterpret_cast<const int64_t*>(info_at), scn = scratch->numel();
+  LAUNCH("pie_hip_attention_shared",
+         lib.pie_hip_attention_shared(qp, q->stride(0), q->stride(1), c.k, c.v, c.page, c.slot, c.head, c.pages, pxp,
+                                      ipp, ixp, llp, T, Hq, Hkv, D, P, (float)scale, plp, info, scp, scn, op,
+                                      out.stride(0), out.stride(1), lse.p, st));
+  return give_pair(a[4], out, a[5], lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// merge_states(parts, lses, out, lse)
+PyObject* merge_states(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  SERVE(n == 4 && !modes_active());
+  const at::Tensor *p = bf16(a[0]), *l = tensor(a[1], at::kFloat);
+  const bool is_bf16 = p != nullptr;
+  if (!p) p = tensor(a[0], at::kFloat);
+  SERVE(p && l && p->dim() == 4 && l->dim() == 3 && p->device() == l->device() && p->numel() > 0 &&
+        l->size(0) == p->size(0) && l->size(1) == p->size(1) && l->size(2) == p->size(2) && p->stride(3) == 1);
+  const int64_t S = p->size(0), T = p->size(1), H = p->size(2), D = p->size(3);
+  at::Tensor out, lse;
+  const auto given = [&](PyObject* o, at::ScalarType dtype, at::IntArrayRef sizes, at::Tensor& t) {
+    if (o == Py_None) {
+      t = at::empty(sizes, at::TensorOptions().dtype(dtype).device(p->device()));
+      return t.unsafeGetTensorImpl()->has_storage() && !t.key_set().has_any(kTransforms);
+    }
+    const at::Tensor* g = tensor(o, dtype);
+    if (!g || g->device() != p->device() || g->sizes() != sizes) return false;
+    t = *g;
+    return true;
+  };
+  SERVE(given(a[2], p->scalar_type(), {T, H, D}, out) && out.stride(2) == 1 && given(a[3], at::kFloat, {T, H}, lse));
+  const c10::DeviceGuard guard(p->device());
+  void *st = stream_of(*p), *pp = p->data_ptr(), *op = out.data_ptr();
+  float *lp = ptr<float>(*l), *ep = ptr<float>(lse);
+  LAUNCH("pie_hip_attention_merge_states",
+         lib.pie_hip_attention_merge_states(pp, is_bf16, p->stride(0), p->stride(1), p->stride(2), lp, l->stride(0),
+                                            l->stride(1), l->stride(2), S, T, H, D, op, out.stride(0), out.stride(1), ep,
+                                            lse.stride(0), lse.stride(1), st));
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, give(a[2], out));
+  PyTuple_SET_ITEM(pair, 1, give(a[3], lse));
+  return pair;
   END_HANDLE_TH_ERRORS
 }
 
@@ -473,6 +604,8 @@ PyMethodDef methods[] = {FAST(bind),
                          FAST(qk_rms_norm_rope_append),
                          FAST(attention_decode),
                          FAST(attention_prefill),
+                         FAST(attention_shared),
+                         FAST(merge_states),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods};
 
