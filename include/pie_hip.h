@@ -523,7 +523,7 @@ int pie_hip_attention_prefill_lse(const pie_bf16* q, int64_t q_tok_stride, int64
  *
  * pie_hip_attention_shared_plan runs on the host over host tables and writes the work list (`plan`, int32
  * words that the caller copies to the device; NULL: only info is filled, info[0] = its words) and
- * info[16] for the run (info[1] = the scratch bytes it needs, at most scratch_bytes). num_cus: the
+ * info[17] for the run (info[1] = the scratch bytes it needs, at most scratch_bytes). num_cus: the
  * device's compute units (0: 256). The run reads prefix_indices and the suffix tables on the device: with
  * one query token per request one plan, and one captured run, serve suffixes of any length (the lengths
  * at plan time only steer how the work is cut); with qo_indptr the plan holds for its own lengths.

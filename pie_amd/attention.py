@@ -529,7 +529,7 @@ class BatchSharedPrefixAttentionWrapper:
             device[arg] = _not_empty(t.to(dev))
         ws_bytes = self._workspace.numel() * self._workspace.element_size()
         scratch_off = -self._workspace.data_ptr() % 16
-        info = (C.c_int64 * 16)()
+        info = (C.c_int64 * 17)()
         ptr = lambda arg: host[arg].data_ptr() if arg in host else None
         args = (ptr("group_indptr"), groups, ptr("prefix_indptr"), ptr("prefix_last_page_len"), ptr("qo_indptr"),
                 ptr("paged_kv_indptr"), ptr("paged_kv_last_page_len"), batch, page_size, num_qo_heads, num_kv_heads,
@@ -540,7 +540,7 @@ class BatchSharedPrefixAttentionWrapper:
         scratch = self._workspace.view(-1).view(torch.uint8)[scratch_off: scratch_off + info[1]]
         self._plan = dict(indptr=device["paged_kv_indptr"], indices=device["paged_kv_indices"],
                           last_page_len=device["paged_kv_last_page_len"], prefix_indices=device["prefix_indices"],
-                          T=info[8], Hq=num_qo_heads, Hkv=num_kv_heads, D=head_dim, P=page_size,
+                          T=info[9], Hq=num_qo_heads, Hkv=num_kv_heads, D=head_dim, P=page_size,
                           plan=torch.from_numpy(words).to(dev), info=info, info_at=C.addressof(info), scratch=scratch,
                           sm_scale=(1.0 / math.sqrt(head_dim)) if sm_scale is None else float(sm_scale))
 

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void attn_decode_kernel(
   __shared__ __attribute__((aligned(16))) char smem[decode_smem<D>()];
   __shared__ int32_t ptab[kPageWin];
   decode_unit<D, FIRST>(smem, ptab, blockIdx.x, q, q_ts, q_hs, kv, B, G, Hq, scale_log2, splits, window_left, first,
-                        false, out, o_ts, o_hs, part_o, part_lse, sinks, lse);
+                        out, o_ts, o_hs, part_o, part_lse, sinks, lse);
 }
 
 // Combines the partial results of each (request, head): one work group per request and 512 / D

@@ -385,12 +385,12 @@ constexpr int decode_smem() {
 }
 
 // One decode unit: split j of request b for kv head kvh, as above, for the launch's unit `unit`.
-// With one split (and no `partial`) it writes the output; otherwise an fp32 partial output and its
+// With one split it writes the output; otherwise an fp32 partial output and its
 // log2-sum-exp to rows (b * splits + j) * Hq + head of part_o / part_lse.
 template <int D, bool FIRST>
 __device__ __forceinline__ void decode_unit(
     char* smem, int32_t* ptab, int unit, const uint16_t* __restrict__ q, int64_t q_ts, int64_t q_hs, const PagedKV& kv,
-    int B, int G, int Hq, float scale_log2, int splits, int window_left, int first, bool partial,
+    int B, int G, int Hq, float scale_log2, int splits, int window_left, int first,
     uint16_t* __restrict__ out, int64_t o_ts, int64_t o_hs, float* __restrict__ part_o, float* __restrict__ part_lse,
     const float* __restrict__ sinks, float* __restrict__ lse) {
   using W = WaveAttn<D>;
@@ -424,7 +424,7 @@ __device__ __forceinline__ void decode_unit(
   } else {
     split_range(kv_len - ws, splits, j, kv0, kv1);
   }
-  const bool whole = splits == 1 && !partial;
+  const bool whole = splits == 1;
   if (!whole && kv0 >= kv1) return;  // an empty split: the merge does not read it
   if constexpr (!FIRST) {
     kv0 += ws;

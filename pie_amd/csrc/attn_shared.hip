@@ -8,10 +8,11 @@
 // MI355X mapping. A prefix read once per request costs its bytes n times over; read for the group it is
 // a matrix product of all the group's query rows (tokens x the kv head's query heads) with the prefix,
 // cut into items of 128 rows over a piece of the prefix (prefill_item), which MFMA bounds at many rows
-// and HBM at few. The suffixes are private: a decode step's are streamed by decode units (decode_unit),
-// bound by HBM, runs of several query tokens per request are causal prefill items. Both kinds run in one
-// launch, the prefix's work groups first: they use the matrix cores while the suffixes' use the memory.
-// Every part leaves an fp32 partial result, joined by a second launch (attn_shared_merge_kernel).
+// and HBM at few. The suffixes are private: a decode step's, and prefixes that at most 16 rows share, are
+// streamed by stream units (below), bound by HBM; runs of several query tokens per request are causal
+// prefill items. All run in one launch, the prefill items' work groups first: they use the matrix cores
+// while the others use the memory. Every part leaves an fp32 partial result, joined by a second launch
+// (attn_shared_merge_kernel).
 #include <string.h>
 
 #include <algorithm>
@@ -22,8 +23,9 @@
 
 namespace pie {
 
-// The plan on the device: prefix items and (several query tokens per request) suffix items of
-// kItemWords each, then kTokenWords per query token.
+// The plan on the device: kItemWords each for the prefill items of prefixes and (several query tokens
+// per request) of suffixes, then for the stream items of prefixes; then kTokenWords per query token; then,
+// in a decode step, the requests, longest suffix first.
 // Item: first row, first query token, query tokens, kv length, first page-table slot, start and length of
 // the piece, first partial row of kv head 0 (kv head h: + h * rows of the run).
 // Query token: {first partial row, rows of the run, the token's first row in the run, pieces} of its
@@ -38,47 +40,153 @@ struct SharedArgs {
   PagedKV kv;                     // the suffixes' pages
   const int32_t* prefix_indices;  // the prefixes' page ids
   const int32_t* plan;
-  int G, Hq, Hkv, prefix_items, suffix_items, B, splits;
+  const int32_t* order;           // decode: the requests in the order they are worked on
+  int G, Hq, Hkv, prefix_items, suffix_items, stream_items, B, splits, heads;
   float scale_log2;
   float *part_o, *part_lse;
   int64_t suffix_row;  // decode: first partial row of the suffixes
 };
 
-// Work groups of a list of items: one per (item, kv head), padded to the XCDs.
-__host__ __device__ __forceinline__ int shared_blocks(int items, int Hkv) { return (items * Hkv + 7) / 8 * 8; }
-
-// The kernel's arguments, loaded where they are used: one branch's need not stay in scalar registers
-// over the other's (the decode units' spilled 36 of them at head dim 64).
-__device__ __forceinline__ SharedArgs branch_args(const SharedArgs& a) {
-#ifdef PIE_HOST_EMULATION
-  return a;
-#else
-  typedef const __attribute__((address_space(4))) uint32_t* words_t;
-  words_t p = (words_t)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  union { uint32_t w[sizeof(SharedArgs) / 4]; SharedArgs a; } u;
+// A stream unit: at most 16 query rows (row n: query token q0 + n / G, head n % G of the kv head's group)
+// over positions [kv0, kv1) of a run of pages, for one or two (`heads`) adjacent kv heads. The four waves
+// are shared out among the heads; a head's waves take its tiles in turn and meet in LDS. With two heads the
+// page table and the set-up are paid once for both and the waves read the heads' rows of a token side by
+// side (four heads gain nothing more). A wave loads its next tile as soon as it has the current one's V in
+// registers and its scores. HBM bounds it.
+struct StreamRun {
+  int q0, rows, kv0, kv1, page0, kvh0;
+  const int32_t* indices;
+  int64_t part_row;  // of kv head 0, row 0; head h: + h * rows
+};
+template <int D>
+__device__ __forceinline__ void stream_unit(char* smem, int32_t* ptab, const StreamRun& run, const uint16_t* __restrict__ q,
+                                            int64_t q_ts, int64_t q_hs, const PagedKV& kv, int G, int heads,
+                                            float scale_log2, float* __restrict__ part_o, float* __restrict__ part_lse) {
+  using W = WaveAttn<D>;
+  constexpr int kVtile = kTileTokens * D;  // elements of one V tile
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int share = 4 / heads, phase = w / heads, kvh = run.kvh0 + w % heads;  // waves of a head, this one's place
+  W st;
+  st.init();
+  {
+    const bool valid = n < run.rows;
+    const int tok = valid ? n / G : 0, hg = valid ? n - tok * G : 0;
+    const uint16_t* qp = q + (int64_t)(run.q0 + tok) * q_ts + (int64_t)(kvh * G + hg) * q_hs;
 #pragma unroll
-  for (unsigned i = 0; i < sizeof(SharedArgs) / 4; ++i) u.w[i] = p[i];
-  return u.a;
-#endif
+    for (int s = 0; s < W::NS; ++s) {
+      const u32x4_t z = {0u, 0u, 0u, 0u};
+      st.qb[s] = valid ? ld16v(qp + 8 * (4 * s + g)) : z;
+    }
+  }
+  uint16_t* vt = reinterpret_cast<uint16_t*>(smem) + w * kVtile;
+  const int step = share * kTileTokens;
+  const int win = max(kTileTokens, (kPageWin - 2) * kv.page_size / kTileTokens * kTileTokens);
+  for (int wt0 = run.kv0; wt0 < run.kv1; wt0 += win) {
+    const int wt1 = min(run.kv1, wt0 + win);
+    const int lp0 = (int)kv.pdiv.div((uint32_t)wt0);
+    const int npg = (int)kv.pdiv.div((uint32_t)(wt1 - 1)) - lp0 + 1;
+    __syncthreads();  // the previous window's lookups are done
+    for (int i = threadIdx.x; i < npg; i += 256) ptab[i] = run.indices[run.page0 + lp0 + i];
+    __syncthreads();
+    KVTile<D> t;
+    int t0 = wt0 + kTileTokens * phase;
+    if (t0 < wt1) t.load(kv, ptab, lp0, KeptMap{}, t0, wt1, kvh, lane, vt);
+    for (; t0 < wt1; t0 += step) {
+      u32x4_t vb[W::NB];
+      float s[2][4], a[4];
+      bool rescale;
+      wait_vmcnt<0>();
+      st.read_v(vt, lane, vb);
+      st.scores(t.ka, t.vmask(lane), scale_log2, s);
+      wait_lgkmcnt0();
+      __builtin_amdgcn_sched_barrier(0);  // (loads moved up would need registers of their own)
+      if (t0 + step < wt1) t.load(kv, ptab, lp0, KeptMap{}, t0 + step, wt1, kvh, lane, vt);
+      __builtin_amdgcn_sched_barrier(0);
+      const u32x4_t pa = st.softmax(s, lane, a, rescale);
+#pragma unroll
+      for (int nb = 0; nb < W::NB; ++nb) st.pv(pa, vb[nb], a, rescale, nb);
+    }
+  }
+  // the waves' results through LDS: m[4][16], l[4][16], o[4][16][D] (fp32); wave p * heads + h is part p of
+  // head h
+  const float lsum = st.row_sum(lane);
+  __syncthreads();
+  float* ms = reinterpret_cast<float*>(smem);
+  float* ls = ms + 4 * 16;
+  float* os = ls + 4 * 16;
+  if (g == 0) { ms[w * 16 + n] = st.m; ls[w * 16 + n] = lsum; }
+#pragma unroll
+  for (int nb = 0; nb < W::NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * g + i < run.rows) os[(w * 16 + 4 * g + i) * D + 16 * nb + n] = st.o[nb][i];
+  __syncthreads();
+  constexpr int CH = D / 8;
+  for (int u = threadIdx.x; u < heads * run.rows * CH; u += 256) {
+    const int hr = u / CH, c = u % CH, h = hr / run.rows, row = hr - h * run.rows;
+    float M = -INFINITY;
+    for (int p = 0; p < share; ++p) M = fmaxf(M, ms[(p * heads + h) * 16 + row]);
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+    const float ref = M == -INFINITY ? 0.f : M;
+    for (int p = 0; p < share; ++p) {
+      const int x = (p * heads + h) * 16 + row;
+      const float f = fast_exp2(ms[x] - ref);
+      L = fmaf(ls[x], f, L);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(os[x * D + 8 * c + e], f, acc[e]);
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const int64_t r = run.part_row + (int64_t)(run.kvh0 + h) * run.rows + row;
+    float4* dst = reinterpret_cast<float4*>(part_o + r * D + 8 * c);
+    dst[0] = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    dst[1] = make_float4(acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
+    if (c == 0) part_lse[r] = L > 0.f ? M + log2f(L) : -INFINITY;
+  }
 }
 
-// RAGGED: several query tokens per request.
-template <int D, bool RAGGED>
+// Work groups of a list of prefill items: one per (item, kv head), padded to the XCDs.
+__host__ __device__ __forceinline__ int shared_blocks(int items, int Hkv) { return (items * Hkv + 7) / 8 * 8; }
+
+// STREAM: stream units (a decode step, or prefixes of few rows).
+template <int D, bool STREAM>
 __global__ __launch_bounds__(256, prefill_groups<D>()) void attn_shared_kernel(SharedArgs a) {
-  constexpr int kSmem = prefill_smem<D>() > decode_smem<D>() ? prefill_smem<D>() : decode_smem<D>();
+  constexpr int kUnit = STREAM ? decode_smem<D>() : 0, kItem = prefill_smem<D>();
+  constexpr int kSmem = kItem > kUnit ? kItem : kUnit;
   __shared__ __attribute__((aligned(16))) char smem[kSmem];
   __shared__ int32_t ptab[kPageWin];
-  // Items of one kind in prefill_unit's order: each XCD takes a run of them, those of one piece together.
-  const int prefix_blocks = shared_blocks(a.prefix_items, a.Hkv);
-  const bool suffix = (int)blockIdx.x >= prefix_blocks;
-  if (!RAGGED && suffix) {
-    const SharedArgs d = branch_args(a);
-    decode_unit<D, false>(smem, ptab, (int)blockIdx.x - prefix_blocks, d.q, d.q_ts, d.q_hs, d.kv, d.B, d.G, d.Hq,
-                          d.scale_log2, d.splits, -1, 0, true, nullptr, 0, 0, d.part_o + d.suffix_row * D,
-                          d.part_lse + d.suffix_row, nullptr, nullptr);
+  // Prefill items of one kind in prefill_unit's order: each XCD takes a run of them, those of one piece together.
+  const int prefix_blocks = shared_blocks(a.prefix_items, a.Hkv), item_blocks = prefix_blocks + shared_blocks(a.suffix_items, a.Hkv);
+  if (STREAM && (int)blockIdx.x >= item_blocks) {
+    const int heads = a.heads, blocks = a.Hkv / heads;
+    const int u = (int)blockIdx.x - item_blocks, hb = u % blocks, v = u / blocks;
+    StreamRun run;
+    run.kvh0 = hb * heads;
+    if (v < a.stream_items) {
+      const int32_t* w = a.plan + kItemWords * (a.prefix_items + a.suffix_items + v);
+      run.q0 = uniform(w[1]);
+      run.rows = uniform(w[2]) * a.G;
+      run.page0 = uniform(w[4]);
+      run.kv0 = uniform(w[5]);
+      run.kv1 = min(uniform(w[3]), run.kv0 + uniform(w[6]));
+      run.part_row = uniform(w[7]);
+      run.indices = a.prefix_indices;
+    } else {
+      const int r = (v - a.stream_items) / a.splits, j = v - a.stream_items - r * a.splits;
+      const int b = uniform(a.order[r]);
+      split_range(kv_length(a.kv, b), a.splits, j, run.kv0, run.kv1);
+      if (run.kv0 >= run.kv1) return;  // an empty split: the merge does not read it
+      run.q0 = b;
+      run.rows = a.G;
+      run.page0 = a.kv.indptr[b];
+      run.part_row = a.suffix_row + (int64_t)(b * a.splits + j) * a.Hq;
+      run.indices = a.kv.indices;
+    }
+    stream_unit<D>(smem, ptab, run, a.q, a.q_ts, a.q_hs, a.kv, a.G, heads, a.scale_log2, a.part_o, a.part_lse);
     return;
   }
+  const bool suffix = (int)blockIdx.x >= prefix_blocks;
   const int n = suffix ? a.suffix_items : a.prefix_items, x = (int)blockIdx.x - (suffix ? prefix_blocks : 0);
   const int per = (n * a.Hkv + 7) / 8, u = (x & 7) * per + (x >> 3);
   if (u >= n * a.Hkv) return;  // padding work group
@@ -130,12 +238,11 @@ __global__ __launch_bounds__(256) void attn_shared_merge_kernel(SharedArgs a, co
 template <int D>
 static void launch_shared(hipStream_t st, const SharedArgs& a, int T, int max_parts, const int32_t* tokens,
                           uint16_t* out, int64_t o_ts, int64_t o_hs, float* lse) {
-  const int prefix = shared_blocks(a.prefix_items, a.Hkv);
-  if (a.splits)
-    hipLaunchKernelGGL((attn_shared_kernel<D, false>), dim3(prefix + a.B * a.splits * a.Hkv), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((attn_shared_kernel<D, true>), dim3(prefix + shared_blocks(a.suffix_items, a.Hkv)), dim3(256), 0,
-                       st, a);
+  const int items = shared_blocks(a.prefix_items, a.Hkv) + shared_blocks(a.suffix_items, a.Hkv);
+  const int streams = (a.stream_items + a.B * a.splits) * (a.Hkv / a.heads);
+  if (items + streams)
+    hipLaunchKernelGGL((streams ? attn_shared_kernel<D, true> : attn_shared_kernel<D, false>), dim3(items + streams),
+                       dim3(256), 0, st, a);
   hipLaunchKernelGGL((max_parts <= 4 ? attn_shared_merge_kernel<D, 1> : attn_shared_merge_kernel<D, 8>),
                      dim3(T, (a.Hq + 512 / D - 1) / (512 / D)), dim3(256), 0, st, a, tokens, out, o_ts, o_hs, lse);
 }
@@ -146,12 +253,17 @@ using namespace pie;
 
 // info[]: what a run needs of its plan, and what it checks against its own arguments.
 enum {
-  kInfoWords, kInfoScratch, kInfoPrefixItems, kInfoSuffixItems, kInfoTokensWord, kInfoSplits, kInfoSuffixRow,
-  kInfoMaxParts, kInfoTokens, kInfoBatch, kInfoHq, kInfoHkv, kInfoDim, kInfoPage, kInfoPrefixSlots, kInfoRows
+  kInfoWords, kInfoScratch, kInfoPrefixItems, kInfoSuffixItems, kInfoStreamItems, kInfoTokensWord, kInfoSplits,
+  kInfoSuffixRow, kInfoMaxParts, kInfoTokens, kInfoBatch, kInfoHq, kInfoHkv, kInfoDim, kInfoPage, kInfoRows,
+  kInfoHeads
 };
 
-// The shortest piece of a prefix or suffix: below it a work group is mostly set-up.
-constexpr int64_t kSharedMinChunk = 256;
+// The shortest pieces, in kv tokens, of a prefill item and of a stream unit: below them a work group is mostly
+// set-up (22 requests of at most 96 tokens behind 742: 18 us, 20 with prefill items of 512; four behind 600:
+// 12.9 us, 14.2 with stream units of 256).
+constexpr int64_t kMinPrefill = 256, kMinStream = 128;
+// Query rows of a kv head that a stream unit holds.
+constexpr int64_t kStreamRows = 16;
 
 static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_t* prefix_indptr,
                        const int32_t* prefix_last, const int32_t* qo_indptr, const int32_t* kv_indptr,
@@ -161,13 +273,15 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
   PIE_REQUIRE(group_indptr && prefix_indptr && prefix_last && kv_indptr && kv_last && info, "%s: null argument", what);
   PIE_REQUIRE(groups >= 0 && groups <= (1 << 24) && batch >= 0 && batch <= (1 << 24) && P > 0 && P <= 65536,
               "%s: bad groups %lld / batch %lld / page_size %lld", what, (long long)groups, (long long)batch, (long long)P);
-  PIE_REQUIRE(Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq % Hkv == 0 && Hq <= 65535 && (qo_indptr || Hq / Hkv <= 16),
+  PIE_REQUIRE(Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq % Hkv == 0 && Hq <= 65535 && (qo_indptr || Hq / Hkv <= kStreamRows),
               "%s: need num_qo_heads = G * num_kv_heads (got %lld / %lld), G <= 16 for one query token per request", what,
               (long long)Hq, (long long)Hkv);
   PIE_REQUIRE(D == 64 || D == 128 || D == 256, "%s: head_dim %lld not in {64, 128, 256}", what, (long long)D);
   PIE_REQUIRE(group_indptr[0] == 0 && group_indptr[groups] == batch, "%s: group_indptr must run from 0 to the batch size %lld",
               what, (long long)batch);
-  const int64_t G = Hq / Hkv, slots = (D == 256 ? prefill_groups<256>() : prefill_groups<128>()) * (num_cus > 0 ? num_cus : 256);
+  const int64_t G = Hq / Hkv;
+  const int64_t cus = num_cus > 0 ? num_cus : 256;
+  const int64_t slots = (D == 256 ? prefill_groups<256>() : prefill_groups<128>()) * cus;
   // a run of cached tokens: its length, or -1 for a bad table
   const auto length = [&](const int32_t* indptr, const int32_t* last, int64_t i) -> int64_t {
     const int64_t np = (int64_t)indptr[i + 1] - indptr[i];
@@ -175,18 +289,20 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
     if (np == 0) return 0;
     if (last[i] < 0 || last[i] > P) return -1;
     const int64_t n = (np - 1) * P + last[i];
-    return n < 0x7fffff00ll ? n : -1;
+    return n < 0x7ffff000ll ? n : -1;  // (a tile past the end still has an int position)
   };
   const auto first_token = [&](int64_t b) -> int64_t { return qo_indptr ? qo_indptr[b] : b; };
   PIE_REQUIRE(first_token(0) == 0, "%s: qo_indptr must start at 0", what);
-  struct Run { int64_t len, q0, tokens, page0; };
+  // A run of cached tokens and the query tokens that read it. tiles: its prefill items per piece, 0: streamed.
+  struct Run { int64_t len, q0, tokens, page0, tiles; };
   std::vector<Run> prefix((size_t)groups), suffix((size_t)batch);
-  int64_t total = 0, longest = 0, longest_suffix = 0;  // kv tokens that work groups walk, over all kv heads
+  const auto tiles = [&](int64_t tokens) { return (tokens * G + kPrefillRows - 1) / kPrefillRows; };
+  int64_t total = 0, longest = 0, longest_suffix = 0;  // total: kv tokens that work groups walk, over all kv heads
   for (int64_t b = 0; b < batch; ++b) {
     const int64_t n = length(kv_indptr, kv_last, b), qo = first_token(b + 1) - first_token(b);
     PIE_REQUIRE(n >= 0 && qo >= 0 && qo * G < 0x7fffff00ll, "%s: bad table at request %lld", what, (long long)b);
-    suffix[(size_t)b] = Run{n, first_token(b), qo, kv_indptr[b]};
-    total += n * (qo_indptr ? (qo * G + kPrefillRows - 1) / kPrefillRows : 1) * Hkv;
+    suffix[(size_t)b] = Run{n, first_token(b), qo, kv_indptr[b], qo_indptr ? tiles(qo) : 0};
+    total += n * (qo_indptr ? tiles(qo) : 1) * Hkv;
     longest_suffix = std::max(longest_suffix, n);
   }
   for (int64_t g = 0; g < groups; ++g) {
@@ -195,57 +311,83 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
                 "%s: bad table at group %lld", what, (long long)g);
     const int64_t q0 = first_token(group_indptr[g]), tokens = first_token(group_indptr[g + 1]) - q0;
     PIE_REQUIRE(tokens * G < 0x7fffff00ll, "%s: group %lld has too many query tokens", what, (long long)g);
-    prefix[(size_t)g] = Run{n, q0, tokens, prefix_indptr[g]};
-    total += n * ((tokens * G + kPrefillRows - 1) / kPrefillRows) * Hkv;
+    prefix[(size_t)g] = Run{n, q0, tokens, prefix_indptr[g], tokens * G <= kStreamRows ? 0 : tiles(tokens)};
+    total += n * tiles(tokens) * Hkv;
     if (tokens) longest = std::max(longest, n);
   }
   const int64_t T = first_token(batch);
   PIE_REQUIRE(T < (1 << 27) && T * Hq < 0x7fffff00ll, "%s: too many query tokens", what);
-  // Pieces of equal length near every work group's share of the launch; longer ones where the scratch or
-  // the partial rows' count does not allow it.
-  int64_t target = std::max(kSharedMinChunk, (total + slots - 1) / slots);
-  const auto piece_len = [&](int64_t len) {
-    const int64_t n = std::max<int64_t>(1, (len + target - 1) / target);
-    return std::max<int64_t>(64, ((len + n - 1) / n + 63) / 64 * 64);  // whole tiles
+  // Pieces of equal length near a work group's share of the launch, which for a prefill item is of one kv
+  // head's tokens, for a stream unit of `heads` heads'.
+  int64_t share = total / slots, heads = 1;
+  const auto target = [&](const Run& r) {
+    return r.tiles ? std::max(kMinPrefill, share) : std::max(kMinStream, share / heads);
   };
-  const auto pieces = [&](int64_t len) { return (len + piece_len(len) - 1) / piece_len(len); };
-  int64_t rows = 0, items = 0, suffix_items = 0, splits = 0, max_parts = 0;
-  for (;; target *= 2) {
-    rows = items = suffix_items = max_parts = 0;
+  const auto piece_len = [&](const Run& r) {
+    const int64_t n = std::max<int64_t>(1, (r.len + target(r) - 1) / target(r));
+    return std::max<int64_t>(64, ((r.len + n - 1) / n + 63) / 64 * 64);  // whole tiles
+  };
+  const auto pieces = [&](const Run& r) { return r.tokens ? (r.len + piece_len(r) - 1) / piece_len(r) : 0; };
+  int64_t rows, prefix_rows, items, suffix_items, stream_items, splits, max_parts, streams;
+  const auto lay_out = [&] {
+    rows = items = suffix_items = stream_items = splits = max_parts = 0;
     for (const Run& r : prefix) {
-      rows += pieces(r.len) * r.tokens * Hq;
-      items += pieces(r.len) * ((r.tokens * G + kPrefillRows - 1) / kPrefillRows);
-      if (r.tokens) max_parts = std::max(max_parts, pieces(r.len));
+      rows += pieces(r) * r.tokens * Hq;
+      if (r.tiles) items += pieces(r) * r.tiles;
+      else stream_items += pieces(r);
+      max_parts = std::max(max_parts, pieces(r));
     }
-    const int64_t prefix_rows = rows;
+    prefix_rows = rows;
     if (qo_indptr) {
       int64_t most = 0;
       for (const Run& r : suffix) {
-        const int64_t n = std::max<int64_t>(1, pieces(r.len));
+        const int64_t n = std::max<int64_t>(1, pieces(r));
         rows += n * r.tokens * Hq;
-        suffix_items += n * ((r.tokens * G + kPrefillRows - 1) / kPrefillRows);
+        suffix_items += n * r.tiles;
         most = std::max(most, n);
       }
       max_parts += most;
     } else {
-      // (a decode step's suffixes grow under one plan: room for 512 tokens more)
-      splits = std::min<int64_t>(64, pieces(longest_suffix + 512));
+      // A decode step's suffixes grow under one plan: as many splits as 512 tokens more ask for, as long as
+      // the launch holds them all at once (242 requests of at most 26 tokens, 2 kv heads: 14.8 us with one
+      // split, 15.9 with five, four of them empty).
+      const auto of = [&](int64_t len) { return pieces(Run{len, 0, 1, 0, 0}); };
+      const int64_t room = slots / std::max<int64_t>(1, batch * (Hkv / heads));
+      splits = std::min<int64_t>(64, std::max({(int64_t)1, of(longest_suffix), std::min(of(longest_suffix + 512), room)}));
       rows += batch * splits * Hq;
       max_parts += splits;
     }
-    const bool fits = rows < 0x7fffff00ll && rows * (D + 1) * 4 <= scratch_max && (items + suffix_items) * Hkv < 0x7fffff00ll &&
-                      batch * splits * Hkv + (items + suffix_items) * Hkv < 0x7fffff00ll;
-    info[kInfoSuffixRow] = prefix_rows;
-    if (fits) break;
-    PIE_REQUIRE(target < std::max(longest, longest_suffix + 512),
+    streams = (stream_items + batch * splits) * (Hkv / heads);
+  };
+  lay_out();
+  // More stream units than the launch holds at once: two kv heads to each (256 requests behind 16000 tokens,
+  // 8 kv heads: 155 us against 167; 4 behind 600, which leave CUs idle: 14.5 us against 12.9).
+  if (Hkv % 2 == 0 && streams > slots) {
+    heads = 2;
+    lay_out();
+  }
+  // More prefill items than CUs: twice as long ones. Two at once on a CU share its matrix cores and end no
+  // sooner than one of both, with twice the partial results (23 requests of up to 13 tokens behind 5000: 33 us
+  // against 40; fewer items, 61 requests of 16 heads behind 5000, are the worse for it: 45 us against 37).
+  if ((items + suffix_items) * Hkv > cus) {
+    share *= 2;
+    lay_out();
+  }
+  // Longer pieces where the scratch or the partial rows' count does not allow these.
+  while (rows >= 0x7fffff00ll || rows * (D + 1) * 4 > scratch_max || (items + suffix_items) * Hkv + streams >= 0x7fffff00ll) {
+    PIE_REQUIRE(share < std::max(longest, longest_suffix + 512) * heads,
                 "%s: the partial results need %lld bytes of workspace, have %lld", what, (long long)(rows * (D + 1) * 4),
                 (long long)scratch_max);
+    share = std::max(share, kMinStream) * 2;
+    lay_out();
   }
-  const int64_t tokens_word = kItemWords * (items + suffix_items), words = tokens_word + kTokenWords * T;
+  const int64_t tokens_word = kItemWords * (items + suffix_items + stream_items);
+  const int64_t words = tokens_word + kTokenWords * T + (qo_indptr ? 0 : batch);
   info[kInfoWords] = words;
   info[kInfoScratch] = rows * (D + 1) * 4;
   info[kInfoPrefixItems] = items;
   info[kInfoSuffixItems] = suffix_items;
+  info[kInfoStreamItems] = stream_items;
   info[kInfoTokensWord] = tokens_word;
   info[kInfoSplits] = splits;
   info[kInfoMaxParts] = max_parts;
@@ -255,21 +397,23 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
   info[kInfoHkv] = Hkv;
   info[kInfoDim] = D;
   info[kInfoPage] = P;
-  info[kInfoPrefixSlots] = groups ? prefix_indptr[groups] : 0;
+  info[kInfoSuffixRow] = prefix_rows;
   info[kInfoRows] = rows;
+  info[kInfoHeads] = heads;
   if (!plan) return PIE_HIP_OK;
   PIE_REQUIRE(capacity >= words, "%s: needs %lld words, capacity %lld", what, (long long)words, (long long)capacity);
-  int32_t *it = plan, *tok = plan + tokens_word;
+  int32_t *it = plan, *stream = plan + kItemWords * (items + suffix_items), *tok = plan + tokens_word;
   int64_t row = 0;
   // the items of a run in order of pieces, and the part of its query tokens' words
   const auto put = [&](const Run& r, int64_t n, int at) {
-    const int64_t chunk = piece_len(r.len), run_rows = r.tokens * G;
+    const int64_t chunk = piece_len(r), run_rows = r.tokens * G;
+    int32_t*& to = r.tiles ? it : stream;
     for (int64_t s = 0; s < n; ++s)
-      for (int64_t r0 = 0; r0 < run_rows; r0 += kPrefillRows) {
+      for (int64_t r0 = 0; r0 < run_rows; r0 += kPrefillRows) {  // (a streamed run has rows of one tile at most)
         const int32_t w[kItemWords] = {(int32_t)r0, (int32_t)r.q0, (int32_t)r.tokens, (int32_t)r.len, (int32_t)r.page0,
                                        (int32_t)(s * chunk), (int32_t)chunk, (int32_t)(row + s * Hkv * run_rows + r0)};
-        memcpy(it, w, sizeof(w));
-        it += kItemWords;
+        memcpy(to, w, sizeof(w));
+        to += kItemWords;
       }
     for (int64_t i = 0; i < r.tokens; ++i) {
       const int32_t w[4] = {(int32_t)row, (int32_t)run_rows, (int32_t)(i * G), (int32_t)n};
@@ -277,14 +421,19 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
     }
     row += n * run_rows * Hkv;
   };
-  for (const Run& r : prefix) put(r, pieces(r.len), 0);
+  for (const Run& r : prefix) put(r, pieces(r), 0);
   for (int64_t b = 0; b < batch; ++b) {
     if (qo_indptr) {
-      put(suffix[(size_t)b], std::max<int64_t>(1, pieces(suffix[(size_t)b].len)), 4);
+      put(suffix[(size_t)b], std::max<int64_t>(1, pieces(suffix[(size_t)b])), 4);
     } else {
       const int32_t w[4] = {(int32_t)(row + b * splits * Hq), (int32_t)G, 0, (int32_t)-splits};
       memcpy(tok + kTokenWords * b + 4, w, sizeof(w));
     }
+  }
+  if (!qo_indptr) {  // the longest suffixes first, so that the short ones fill the launch's tail
+    int32_t* order = tok + kTokenWords * T;
+    for (int64_t b = 0; b < batch; ++b) order[b] = (int32_t)b;
+    std::stable_sort(order, order + batch, [&](int32_t x, int32_t y) { return suffix[(size_t)x].len > suffix[(size_t)y].len; });
   }
   return PIE_HIP_OK;
 }
@@ -316,7 +465,7 @@ extern "C" int pie_hip_attention_shared(
   const int rc = paged_kv_desc(&a.kv, k_cache, v_cache, page_stride, slot_stride, head_stride, num_pages, kv_indptr,
                                kv_indices, kv_last_page_len, page_size, head_dim, what);
   if (rc) return rc;
-  PIE_REQUIRE(info && (prefix_indices || info[kInfoPrefixItems] == 0), "%s: null argument", what);
+  PIE_REQUIRE(info && (prefix_indices || info[kInfoPrefixItems] + info[kInfoStreamItems] == 0), "%s: null argument", what);
   PIE_REQUIRE(info[kInfoTokens] == num_tokens && info[kInfoHq] == num_qo_heads && info[kInfoHkv] == num_kv_heads &&
                   info[kInfoDim] == head_dim && info[kInfoPage] == page_size,
               "%s: the plan is for %lld tokens, %lld/%lld heads of %lld, pages of %lld", what, (long long)info[kInfoTokens],
@@ -343,14 +492,17 @@ extern "C" int pie_hip_attention_shared(
   a.Hkv = (int)num_kv_heads;
   a.prefix_items = (int)info[kInfoPrefixItems];
   a.suffix_items = (int)info[kInfoSuffixItems];
+  a.stream_items = (int)info[kInfoStreamItems];
   a.B = (int)info[kInfoBatch];
   a.splits = (int)info[kInfoSplits];
+  a.heads = (int)info[kInfoHeads];
   // (prefill_item scales raw scores inside the exponent, where a zero scale would turn -inf into NaN)
   a.scale_log2 = sm_scale == 0.f ? 1e-30f : sm_scale * 1.4426950408889634f;
   a.part_o = static_cast<float*>(scratch);
   a.part_lse = a.part_o + info[kInfoRows] * head_dim;
   a.suffix_row = info[kInfoSuffixRow];
   const int32_t* tokens = plan + info[kInfoTokensWord];
+  a.order = tokens + kTokenWords * num_tokens;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int T = (int)num_tokens, parts = (int)info[kInfoMaxParts];
   switch (head_dim) {

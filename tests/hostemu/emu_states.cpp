@@ -267,7 +267,7 @@ static void case_shared(std::vector<int> sizes, std::vector<int> prefixes, std::
   Buf<int32_t> gb(gi), pb(pre.indptr), px(pre.indices), pl(pre.last), sb(suf.indptr), sx(suf.indices), sl(suf.last), qb(qo);
 
   const int32_t* qp = news.empty() ? nullptr : qb.p;
-  int64_t info[16];
+  int64_t info[17];
   rc_is(pie_hip_attention_shared_plan(gb.p, Gp, pb.p, pl.p, qp, sb.p, sl.p, B, P, Hq, Hkv, D, cus, scratch_max, nullptr, 0, info),
         0, "shared_plan");
   Buf<int32_t> plan(info[0]);
@@ -279,8 +279,8 @@ static void case_shared(std::vector<int> sizes, std::vector<int> prefixes, std::
                                  sb.p, sx.p, sl.p, T, Hq, Hkv, D, P, 1.f / sqrtf((float)D), plan.p, info, scratch.p, info[1],
                                  out.p, Hq * D, D, lse.p, nullptr),
         0, "shared");
-  printf("  prefix items %lld, suffix items %lld, splits %lld, parts <= %lld\n", (long long)info[2], (long long)info[3],
-         (long long)info[5], (long long)info[7]);
+  printf("  prefix items %lld + %lld streamed, suffix items %lld, splits %lld, parts <= %lld\n", (long long)info[2],
+         (long long)info[4], (long long)info[3], (long long)info[6], (long long)info[8]);
   check("shared", out, want, &lse, want_lse);
 }
 
@@ -333,7 +333,7 @@ static void case_merge(int64_t S, int64_t T, int64_t H, int64_t D, bool bf16) {
 static void case_plan() {
   printf("refusals\n");
   int32_t gi[] = {0, 2}, pi[] = {0, 3}, pl[] = {5}, ki[] = {0, 1, 2}, kl[] = {1, 16}, qo[] = {0, 1, 3};
-  int64_t info[16];
+  int64_t info[17];
   const auto plan = [&](int64_t Hq = 8, int64_t Hkv = 2, int64_t D = 128, const int32_t* q = nullptr, int64_t scratch = 1 << 30,
                         int32_t* words = nullptr, int64_t cap = 0) {
     return pie_hip_attention_shared_plan(gi, 1, pi, pl, q, ki, kl, 2, 16, Hq, Hkv, D, 256, scratch, words, cap, info);

@@ -33,7 +33,7 @@ def _plan(ws=1 << 24, heads=HEADS, page=16, **kw):
 def test_a_plan_knows_its_work():
     w = _plan()
     p = w._plan
-    assert p["T"] == 3 and p["info"][2] == 2 and p["plan"].numel() == p["info"][0]
+    assert p["T"] == 3 and p["info"][2] + p["info"][4] == 2 and p["plan"].numel() == p["info"][0]
     assert _plan(qo_indptr=_i32(0, 1, 1, 4))._plan["T"] == 4
     with pytest.raises(RuntimeError, match="GPU"):
         w.run(torch.zeros((3, 8, 128), dtype=torch.bfloat16), torch.zeros((8, 2, 16, 2, 128), dtype=torch.bfloat16))
