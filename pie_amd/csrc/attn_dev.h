@@ -910,21 +910,15 @@ __device__ __forceinline__ void prefill_item(
         next_page = ptab[(int)kv.pdiv.div((uint32_t)wave_tok(tile + 1)) - lp0];
         const uint32_t pg = (unsigned)page < (unsigned)kv.num_pages ? (uint32_t)page : 0u;
         const int64_t base = (int64_t)pg * kv.page_stride + (int64_t)slot0 * kv.slot_stride + (int64_t)kvh * kv.head_stride;
-        const auto kb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kv.k + base), 0, 0x7fffffff, 0x00020000);
-        const auto vb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kv.v + base), 0, 0x7fffffff, 0x00020000);
+        // rows past the end lie behind the buffers' and read as zero (their probability is 0)
+        const int bytes = 2 * ((min(WR, wt1 - tb) - 1) * (int)kv.slot_stride + D);
+        const auto kb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kv.k + base), 0, bytes, 0x00020000);
+        const auto vb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kv.v + base), 0, bytes, 0x00020000);
         const uint32_t ko = (uint32_t)opaque_v((int)koff);
-        uint32_t back[NL];
-#pragma unroll
-        for (int i = 0; i < NL; ++i) back[i] = 0;
-        if (t0 + TT > wt1) {  // the last tile: rows past the end read the last row (their probability is 0)
-#pragma unroll
-          for (int i = 0; i < NL; ++i)
-            back[i] = 2u * (uint32_t)max(0, RPI * i + lane / CH - (wt1 - 1 - tb)) * (uint32_t)kv.slot_stride;
-        }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-          sl.k[i] = __builtin_amdgcn_raw_buffer_load_b128(kb, (int)((ko ^ k_xor(i)) + i * step - back[i]), 0, 0);
-          sl.v[i] = __builtin_amdgcn_raw_buffer_load_b128(vb, (int)((voff ^ v_xor(i)) + i * step - back[i]), 0, 0);
+          sl.k[i] = __builtin_amdgcn_raw_buffer_load_b128(kb, (int)((ko ^ k_xor(i)) + i * step), 0, 0);
+          sl.v[i] = __builtin_amdgcn_raw_buffer_load_b128(vb, (int)((voff ^ v_xor(i)) + i * step), 0, 0);
         }
       } else {
 #pragma unroll
@@ -1069,23 +1063,25 @@ __device__ __forceinline__ void prefill_item(
       }
       float mx = -INFINITY;
       if (!neg) {
-        float mh[4 * H2];
+        // (three-operand maxima in two chains; a tree of two-operand ones takes twice the instructions, since the
+        // products' results are quieted first)
+        float mh[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int h = 0; h < H2; ++h)
+        for (int i = 0; i < 16 * H2; i += 4)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            mh[4 * h + c] = fmaxf(fmaxf(sacc[h][4 * c], sacc[h][4 * c + 1]), fmaxf(sacc[h][4 * c + 2], sacc[h][4 * c + 3]));
-#pragma unroll
-        for (int c = 0; c < 4 * H2; ++c) mx = fmaxf(mx, mh[c]);
+          for (int c = 0; c < 2; ++c)
+            mh[c] = fmaxf(fmaxf(mh[c], sacc[i >> 4][(i & 15) + 2 * c]), sacc[i >> 4][(i & 15) + 2 * c + 1]);
+        mx = fmaxf(mh[0], mh[1]);
       } else {
 #pragma unroll
         for (int h = 0; h < H2; ++h)
 #pragma unroll
           for (int i = 0; i < 16; ++i) mx = fmaxf(mx, -sacc[h][i]);
       }
-      mx = fmaxf(mx, other_half(mx)) * fabsf(scale_log2);
-      // lazy maximum (kLazyMax)
+      mx *= fabsf(scale_log2);
+      // lazy maximum (kLazyMax); the row's other half of the tokens is looked at only where one half exceeds it
       if (__builtin_amdgcn_ballot_w64(mx > m_run + kLazyMax) != 0) {
+        mx = fmaxf(mx, other_half(mx));
         const bool grow = mx > m_run + kLazyMax;
         const float alpha = grow ? fast_exp2(m_run - mx) : 1.f;
         if (grow) m_run = mx;

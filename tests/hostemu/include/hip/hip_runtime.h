@@ -318,16 +318,16 @@ inline float __builtin_amdgcn_sinf(float x) { return (float)sin(6.28318530717958
 inline float __builtin_amdgcn_cosf(float x) { return (float)cos(6.283185307179586 * (double)x); }
 inline float __builtin_amdgcn_fractf(float x) { return x - floorf(x); }
 // Buffer resources: the base address only (no range checks; callers stay in bounds).
-typedef char* __amdgpu_buffer_rsrc_t;
-inline __amdgpu_buffer_rsrc_t __builtin_amdgcn_make_buffer_rsrc(void* p, short, int, int) { return (char*)p; }
+struct __amdgpu_buffer_rsrc_t { char* p; unsigned bytes; };  // (loads past its bytes give zero)
+inline __amdgpu_buffer_rsrc_t __builtin_amdgcn_make_buffer_rsrc(void* p, short, int n, int) { return {(char*)p, (unsigned)n}; }
 typedef unsigned emu_u32x4 __attribute__((ext_vector_type(4)));
 inline emu_u32x4 __builtin_amdgcn_raw_buffer_load_b128(__amdgpu_buffer_rsrc_t r, int off, int soff, int) {
-  emu_u32x4 v;
-  memcpy(&v, r + off + soff, 16);
+  emu_u32x4 v = {0u, 0u, 0u, 0u};
+  if ((unsigned)off < r.bytes) memcpy(&v, r.p + off + soff, 16);
   return v;
 }
 inline void __builtin_amdgcn_raw_buffer_store_b128(emu_u32x4 v, __amdgpu_buffer_rsrc_t r, int off, int soff, int) {
-  memcpy(r + off + soff, &v, 16);
+  if ((unsigned)off < r.bytes) memcpy(r.p + off + soff, &v, 16);
 }
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define hipLaunchKernelGGL(k, g, b, shm, st, ...) emu::launch(k, dim3(g), dim3(b), __VA_ARGS__)
