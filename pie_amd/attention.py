@@ -485,11 +485,12 @@ class BatchSharedPrefixAttentionWrapper:
     qo_indptr[b+1] - qo_indptr[b]. Prefixes and suffixes may be empty.
 
     ``plan`` reads the index arrays on the host (a copy, for GPU tensors). With one query token per
-    request the suffix tables are read on the device by each run: one plan, and one captured run, serve
-    suffixes of any length, whose lengths at plan time only steer how the work is cut. With qo_indptr a
-    plan holds for its own lengths. Partial results live in the workspace from a run's first launch to
-    its second: give wrappers whose runs overlap in time their own (an eager run while another stream's
-    run uses the workspace raises). A captured run keeps the plan it was captured with."""
+    request the suffix tables are read on the device by each run (the caller's, where given as GPU
+    tensors): one plan, and one captured run, serve suffixes of any length, whose lengths at plan time only
+    steer how the work is cut. With qo_indptr a plan holds for its own lengths. Partial results live in the
+    workspace from a run's first launch to its second: give wrappers whose runs overlap in time their own
+    (an eager run while another stream's run uses the workspace raises). A captured run keeps the plan it
+    was captured with, for as long as the wrapper lives: keep both it and the workspace with the graph."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
         if kv_layout not in ("NHD", "HND"):
@@ -518,7 +519,7 @@ class BatchSharedPrefixAttentionWrapper:
                 raise ValueError(f"{name}: {arg} must be {n} int32 values, got {t.dtype} {tuple(t.shape)}")
             host[arg] = t.cpu().contiguous()
         dev = self._workspace.device
-        device = {}
+        device, made = {}, []
         for arg, t, n in (("prefix_indices", prefix_indices, int(host["prefix_indptr"][-1])),
                           ("paged_kv_indices", paged_kv_indices, int(host["paged_kv_indptr"][-1])),
                           ("paged_kv_indptr", paged_kv_indptr, batch + 1),
@@ -527,6 +528,8 @@ class BatchSharedPrefixAttentionWrapper:
                 raise ValueError(f"{name}: {arg} must hold at least {n} contiguous int32 values, got {t.dtype} "
                                  f"{tuple(t.shape)}")
             device[arg] = _not_empty(t.to(dev))
+            if device[arg] is not t:
+                made.append(device[arg])
         ws_bytes = self._workspace.numel() * self._workspace.element_size()
         scratch_off = -self._workspace.data_ptr() % 16
         info = (C.c_int64 * 17)()
@@ -538,10 +541,13 @@ class BatchSharedPrefixAttentionWrapper:
         words = np.empty(max(1, info[0]), dtype=np.int32)
         _lib.call("pie_hip_attention_shared_plan", *args, words.ctypes.data, words.size, info)
         scratch = self._workspace.view(-1).view(torch.uint8)[scratch_off: scratch_off + info[1]]
-        self._plan = dict(indptr=device["paged_kv_indptr"], indices=device["paged_kv_indices"],
+        plan = torch.from_numpy(words).to(dev)
+        # (made, stream: a run on another stream tells the allocator about the memory that a new plan would free)
+        self._plan = dict(made=made + [plan], stream=_stream(plan) if plan.is_cuda else 0,
+                          indptr=device["paged_kv_indptr"], indices=device["paged_kv_indices"],
                           last_page_len=device["paged_kv_last_page_len"], prefix_indices=device["prefix_indices"],
                           T=info[9], Hq=num_qo_heads, Hkv=num_kv_heads, D=head_dim, P=page_size,
-                          plan=torch.from_numpy(words).to(dev), info=info, info_at=C.addressof(info), scratch=scratch,
+                          plan=plan, info=info, info_at=C.addressof(info), scratch=scratch,
                           sm_scale=(1.0 / math.sqrt(head_dim)) if sm_scale is None else float(sm_scale))
 
     def run(self, q: torch.Tensor, paged_kv_cache: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]],
@@ -551,8 +557,13 @@ class BatchSharedPrefixAttentionWrapper:
         p = self._plan
         if p is None:
             raise RuntimeError(f"{name}: plan() must be called before run()")
-        if p["plan"].is_cuda and torch.cuda.is_current_stream_capturing() and not any(k is p for k in self._captured):
-            self._captured.append(p)
+        if p["plan"].is_cuda:
+            if torch.cuda.is_current_stream_capturing():
+                if not any(k is p for k in self._captured):
+                    self._captured.append(p)
+            elif _stream(p["plan"]) != p["stream"]:
+                for t in p["made"]:
+                    t.record_stream(torch.cuda.current_stream(t.device))
         if _lib.fast is not None:
             r = _lib.fast.attention_shared(p, q, paged_kv_cache, self._kv_layout, out, lse if lse is not None else return_lse)
             if r is not None:

@@ -455,6 +455,61 @@ def test_shared_run_on_a_busy_workspace_is_refused(dev):
     _compare(outs[1], want, "second stream")
 
 
+@pytest.mark.parametrize("heads", [(32, 8, 128), (6, 3, 64), (8, 4, 256)])
+def test_many_requests(dev, heads):
+    """More stream units than the device runs at once: two kv heads to a work group, where their number is even;
+    suffixes of every length around the tiles' and pieces' ends."""
+    suffixes = [(37 * b) % 300 for b in range(190)]
+    c, args, kw, q, want = _shared_case(dev, [150, 3, 37], [700, 40, 129], suffixes, None, heads, 16)
+    w = attention.BatchSharedPrefixAttentionWrapper(_ws(dev, 256 << 20))
+    w.plan(*args, *heads, 16)
+    got = w.run(q, c.arg, return_lse=True)
+    _compare(got, want, "many requests")
+    again = w.run(q, c.arg, return_lse=True)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("news", [None, [9, 1, 30, 4]])
+def test_shared_prefix_at_other_scales(dev, news):
+    heads = (32, 8, 128)
+    c, args, kw, q, want = _shared_case(dev, [3, 1], [200, 33], [40, 9, 70, 4], news, heads, 16)
+    w = attention.BatchSharedPrefixAttentionWrapper(_ws(dev))
+    w.plan(*args, *heads, 16, sm_scale=-128 ** -0.5, **kw)
+    _compare(w.run(-q, c.arg, return_lse=True), want, "a negative scale")
+    w.plan(*args, *heads, 16, sm_scale=0.0, **kw)
+    got = w.run(q, c.arg, return_lse=True)
+    w.plan(*args, *heads, 16, **kw)
+    mean = w.run(torch.zeros_like(q), c.arg, return_lse=True)
+    assert torch.equal(got[0], mean[0]) and torch.allclose(got[1], mean[1], rtol=2 ** -22, atol=0)
+
+
+def test_a_plan_outlives_runs_on_other_streams(dev):
+    """A run queued on another stream than its plan's, then a new plan: the first one's memory is not handed
+    out before the run has read it."""
+    heads = (8, 2, 128)
+    c, args, kw, q, want = _shared_case(dev, [40], [900], [3 + b for b in range(40)], None, heads, 16)
+    w = attention.BatchSharedPrefixAttentionWrapper(_ws(dev))
+    w.plan(*(t.cpu() for t in args), *heads, 16)
+    made = [(t.numel(), t.data_ptr()) for t in w._plan["made"]]
+    out, lse = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty(q.shape[:2], device=dev)
+    s = torch.cuda.Stream()
+    w.run(q, c.arg)  # (the kernels are loaded)
+    big = torch.zeros(1 << 28, device=dev)
+    with torch.cuda.stream(s):
+        big.add_(1)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(20):  # some ms before the run
+            big.add_(1)
+        w.run(q, c.arg, out=out, lse=lse)
+    w.plan(*(t.cpu() for t in args), *heads, 16)
+    new = [torch.full((n,), -1, dtype=torch.int32, device=dev) for n, _ in made for _ in range(4)]
+    assert not s.query()  # (the run was still queued)
+    assert not {t.data_ptr() for t in new + w._plan["made"]} & {at for _, at in made}
+    torch.cuda.synchronize()
+    _compare((out, lse), want, "another stream")
+
+
 def test_offsets_past_32_bits(dev):
     """Pages whose elements lie past 2^32 bytes and 2^31 elements of the pool."""
     heads, P = (8, 4, 128), 32
