@@ -489,7 +489,8 @@ class BatchSharedPrefixAttentionWrapper:
     tensors): one plan, and one captured run, serve suffixes of any length, whose lengths at plan time only
     steer how the work is cut. With qo_indptr a plan holds for its own lengths. Partial results live in the
     workspace from a run's first launch to its second: give wrappers whose runs overlap in time their own
-    (an eager run while another stream's run uses the workspace raises). A captured run keeps the plan it
+    (an eager run while another stream's run uses the workspace raises). So does a prefill wrapper's plan, which
+    a run of this one in the same workspace overwrites: plan it again before its next run, or give it its own. A captured run keeps the plan it
     was captured with, for as long as the wrapper lives: keep both it and the workspace with the graph."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
