@@ -526,7 +526,8 @@ int pie_hip_attention_prefill_lse(const pie_bf16* q, int64_t q_tok_stride, int64
  * info[17] for the run (info[1] = the scratch bytes it needs, at most scratch_bytes). num_cus: the
  * device's compute units (0: 256). The run reads prefix_indices and the suffix tables on the device: with
  * one query token per request one plan, and one captured run, serve suffixes of any length (the lengths
- * at plan time only steer how the work is cut); with qo_indptr the plan holds for its own lengths.
+ * at plan time only steer how the work is cut); with qo_indptr the plan holds for its own lengths, and
+ * may need no scratch at all (info[1] = 0).
  * scratch (16-byte aligned) holds partial results from the run's first launch to its second: runs that
  * share it must not overlap. One made while another stream's run uses it, or between another thread's
  * launches, returns PIE_HIP_EBUSY; runs recorded under graph capture are not checked.

@@ -756,14 +756,18 @@ __device__ __forceinline__ float other_half(float v) {
 // kept first tokens, padded to whole tiles, followed by the window's. (18082 tokens in windows of 1024 + 4, 32
 // heads of 128: 353-376 us, 695-740 TFLOP/s over the visible pairs, as the causal prefill of long requests; both
 // ranges' tiles in one loop, with a choice of range per tile, take as long.)
+// JOINT: pre_len tokens of another run of pages (pre_indices from pre_page0 on), which all rows see, come before
+// the item's own kv range.
 struct PrefillItem {
   int b, row0, q0, qo_len, kv_len, page0, off, chunk;
   int64_t part_row;
+  const int32_t* pre_indices = nullptr;
+  int pre_page0 = 0, pre_len = 0;
 };
 template <int D>
 constexpr int prefill_smem() { return 2 * 2 * prefill_tile<D>() * D * 2; }
 
-template <int D, bool FIRST>
+template <int D, bool FIRST, bool JOINT = false>
 __device__ __forceinline__ void prefill_item(
     char* smem, int32_t* ptab, const PrefillItem& it, const uint16_t* __restrict__ q, int64_t q_ts, int64_t q_hs,
     const PagedKV& kv, int G, int n_kv_heads, int kvh, float scale_log2, int mode_in, int window_left, int first_in,
@@ -844,6 +848,7 @@ __device__ __forceinline__ void prefill_item(
   } else {
     kv_begin += it.off;
     kv_end = (int)min((int64_t)kv_end, (int64_t)kv_begin + it.chunk);
+    if constexpr (JOINT) a1 = it.pre_len;
   }
   const int nw = (kv_len + 31) / 32;
   const uint32_t* mword = mode == 2 ? packed + word_off[b] + (int64_t)max(row_tok, 0) * nw : nullptr;
@@ -886,7 +891,7 @@ __device__ __forceinline__ void prefill_item(
   }
   const int win = max(TT, (kPageWin - 2) * kv.page_size / TT * TT);
   // the range of the kept first tokens (FIRST), then the window's
-  bool kept = FIRST && a0 < a1;
+  bool kept = (FIRST || JOINT) && a0 < a1;
   int seg_end = kept ? a1 : kv_end;
   for (int wt0 = kept ? a0 : kv_begin; wt0 < seg_end;) {
     const int wt1 = min(seg_end, wt0 + win);
@@ -896,7 +901,7 @@ __device__ __forceinline__ void prefill_item(
     if (threadIdx.x == 0) window_bad = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < npg; i += NT) {
-      const int pg = kv.indices[page0 + lp0 + i];
+      const int pg = JOINT && kept ? it.pre_indices[it.pre_page0 + lp0 + i] : kv.indices[page0 + lp0 + i];
       ptab[i] = pg;
       if ((unsigned)pg >= (unsigned)kv.num_pages) window_bad = 1;
     }
@@ -967,7 +972,7 @@ __device__ __forceinline__ void prefill_item(
     };
     auto compute = [&](int tile) {
       const int t0 = wt0 + tile * TT;
-      if (t0 > wave_hi) return;  // no row of the wave sees the tile
+      if (JOINT && kept ? !wave_rows : t0 > wave_hi) return;  // no row of the wave sees the tile
       const uint32_t buf = (tile & 1) * 4 * TILE;  // bytes
       const uint32_t kl = (uint32_t)opaque_v((int)(buf + kl0));
       // S^T: token 32h + r32 of the tile against this lane group's 32 rows
@@ -1021,18 +1026,22 @@ __device__ __forceinline__ void prefill_item(
           for (int c = 0; c < 4; ++c) vis[h] |= ((mcur[h] >> (8 * c + 4 * kg)) & 15u) << (4 * c);
         }
       }
-      if (!all_pages_ok || t0 + TT - 1 > wave_lim || t0 < wave_lo) {
+      if (!all_pages_ok || (JOINT && kept ? t0 + TT > wt1 : t0 + TT - 1 > wave_lim || t0 < wave_lo)) {
         uint64_t tv = ~0ull;
         if (!all_pages_ok) {
           bool pok = false;
           if (lane < TT && t0 + lane < wt1) kv_offset_lds(kv, ptab, lp0, t0 + lane, kvh, pok);
           tv = __builtin_amdgcn_ballot_w64(pok);
         }
-        const int hi = row_lim(row_tok) - t0 - 4 * kg;
+        const int hi = (JOINT && kept ? wt1 - 1 : row_lim(row_tok)) - t0 - 4 * kg;
         tv >>= 4 * kg;
-        if constexpr (FIRST) {  // as token bits: [lo, hi] of the window, and the kept ones
-          const int lo = (kept ? 0x7fffffff : row_lo(row_tok)) - t0 - 4 * kg;
-          tv &= (low_bits(hi + 1) & ~low_bits(lo)) | low_bits(min(hi + 1, (kept ? wt1 : first) - t0 - 4 * kg));
+        if constexpr (FIRST || JOINT) {  // as token bits: [lo, hi] of the window, and the kept ones
+          if constexpr (FIRST) {
+            const int lo = (kept ? 0x7fffffff : row_lo(row_tok)) - t0 - 4 * kg;
+            tv &= (low_bits(hi + 1) & ~low_bits(lo)) | low_bits(min(hi + 1, (kept ? wt1 : first) - t0 - 4 * kg));
+          } else {
+            tv &= low_bits(hi + 1);
+          }
 #pragma unroll
           for (int h = 0; h < H2; ++h) {
             uint32_t seen = 0;
@@ -1142,7 +1151,7 @@ __device__ __forceinline__ void prefill_item(
       if (++k >= ntiles) break;
     }
     wt0 += win;
-    if (FIRST && kept && wt0 >= seg_end) {
+    if ((FIRST || JOINT) && kept && wt0 >= seg_end) {
       kept = false;
       wt0 = kv_begin;
       seg_end = kv_end;

@@ -10,8 +10,8 @@
 // cut into items of 128 rows over a piece of the prefix (prefill_item), which MFMA bounds at many rows
 // and HBM at few. The suffixes are private: a decode step's, and prefixes that at most 16 rows share, are
 // streamed by stream units (below), bound by HBM; runs of several query tokens per request are causal
-// prefill items. All run in one launch, the prefill items' work groups first: they use the matrix cores
-// while the others use the memory. Every part leaves an fp32 partial result, joined by a second launch
+// prefill items, which walk a short prefix themselves. All run in one launch, the prefill items' work groups first: they use the matrix cores
+// while the others use the memory. Every other part leaves an fp32 partial result, joined by a second launch
 // (attn_shared_merge_kernel).
 //
 // Measured (32 query and 8 kv heads of 128): 256 requests of 128-1000 tokens behind 16000, 628 MB and 69
@@ -33,12 +33,13 @@ namespace pie {
 // per request) of suffixes, then for the stream items of prefixes; then kTokenWords per query token; then,
 // in a decode step, the requests, longest suffix first.
 // Item: first row, first query token, query tokens, kv length, first page-table slot, start and length of
-// the piece, first partial row of kv head 0 (kv head h: + h * rows of the run).
+// the piece, first partial row of kv head 0 (kv head h: + h * rows of the run; -1: the item walks its
+// group's prefix and then its suffix and writes the output), first page-table slot and length of that prefix.
 // Query token: {first partial row, rows of the run, the token's first row in the run, pieces} of its
 // prefix, and of its suffix. Row r of piece s for kv head h is first + (s * kv heads + h) * rows + r. In a
 // decode step a run of G rows is the request's own and -pieces of them are planned (the device counts
-// those that hold tokens).
-constexpr int kItemWords = 8, kTokenWords = 8;
+// those that hold tokens). -1 prefix pieces: nothing to join, an item wrote the output.
+constexpr int kItemWords = 10, kTokenWords = 8;
 
 struct SharedArgs {
   const uint16_t* q;
@@ -51,6 +52,9 @@ struct SharedArgs {
   float scale_log2;
   float *part_o, *part_lse;
   int64_t suffix_row;  // decode: first partial row of the suffixes
+  uint16_t* out;
+  int64_t o_ts, o_hs;
+  float* lse;
 };
 
 // A stream unit: at most 16 query rows (row n: query token q0 + n / G, head n % G of the kv head's group)
@@ -155,8 +159,9 @@ __device__ __forceinline__ void stream_unit(char* smem, int32_t* ptab, const Str
 // Work groups of a list of prefill items: one per (item, kv head), padded to the XCDs.
 __host__ __device__ __forceinline__ int shared_blocks(int items, int Hkv) { return (items * Hkv + 7) / 8 * 8; }
 
-// STREAM: stream units (a decode step, or prefixes of few rows).
-template <int D, bool STREAM>
+// STREAM: stream units (a decode step, or prefixes of few rows). RAGGED: several query tokens per request; items may
+// walk a prefix and a suffix.
+template <int D, bool STREAM, bool RAGGED>
 __global__ __launch_bounds__(256, prefill_groups<D>()) void attn_shared_kernel(SharedArgs a) {
   constexpr int kUnit = STREAM ? decode_smem<D>() : 0, kItem = prefill_smem<D>();
   constexpr int kSmem = kItem > kUnit ? kItem : kUnit;
@@ -207,11 +212,16 @@ __global__ __launch_bounds__(256, prefill_groups<D>()) void attn_shared_kernel(S
   it.page0 = uniform(w[4]);
   it.off = uniform(w[5]);
   it.chunk = uniform(w[6]);
-  it.part_row = (int64_t)uniform(w[7]) + (int64_t)kvh * (it.qo_len * a.G);
+  const int part_row = uniform(w[7]);
+  it.part_row = part_row < 0 ? -1 : (int64_t)part_row + (int64_t)kvh * (it.qo_len * a.G);
+  it.pre_indices = a.prefix_indices;
+  it.pre_page0 = uniform(w[8]);
+  it.pre_len = uniform(w[9]);
   PagedKV kv = a.kv;
   if (!suffix) kv.indices = a.prefix_indices;
-  prefill_item<D, false>(smem, ptab, it, a.q, a.q_ts, a.q_hs, kv, a.G, a.Hkv, kvh, a.scale_log2, suffix ? 1 : 0, -1, 0,
-                         nullptr, nullptr, nullptr, nullptr, 0, 0, nullptr, a.part_o, a.part_lse, nullptr);
+  prefill_item<D, false, RAGGED>(smem, ptab, it, a.q, a.q_ts, a.q_hs, kv, a.G, a.Hkv, kvh, a.scale_log2, suffix ? 1 : 0,
+                                  -1, 0, nullptr, nullptr, nullptr, a.out, a.o_ts, a.o_hs, nullptr, a.part_o, a.part_lse,
+                                  a.lse);
 }
 
 // Joins the parts of each (query token, head), D / 8 lanes to a head. WIDE (more than kNarrowParts parts): a work
@@ -220,9 +230,7 @@ __global__ __launch_bounds__(256, prefill_groups<D>()) void attn_shared_kernel(S
 // and 5 parts: 11.5 us with the waves sharing, 7.0 with a wave each). HBM and load latency bound it.
 constexpr int kNarrowParts = 8;
 template <int D, bool WIDE>
-__global__ __launch_bounds__(256) void attn_shared_merge_kernel(SharedArgs a, int64_t units, const int32_t* __restrict__ tokens,
-                                                                uint16_t* __restrict__ out, int64_t o_ts, int64_t o_hs,
-                                                                float* __restrict__ lse) {
+__global__ __launch_bounds__(256) void attn_shared_merge_kernel(SharedArgs a, int64_t units, const int32_t* __restrict__ tokens) {
   constexpr int CH = D / 8, HEADS = 64 / CH;
   const int lane = threadIdx.x & 63, per = (a.Hq + HEADS - 1) / HEADS;
   const int64_t u = WIDE ? blockIdx.x : 4 * (int64_t)blockIdx.x + uniform(threadIdx.x >> 6);
@@ -233,6 +241,7 @@ __global__ __launch_bounds__(256) void attn_shared_merge_kernel(SharedArgs a, in
   const int kvh = hl / a.G, hg = hl - kvh * a.G;
   const int32_t* w = tokens + kTokenWords * (int64_t)t;
   const int np = w[3], planned = w[7];
+  if (np < 0) return;  // (of the whole token: every thread of its waves)
   const int room = np + abs(planned);
   const int64_t p0 = (int64_t)w[0] + (int64_t)kvh * w[1] + w[2] + hg, s0 = (int64_t)w[4] + (int64_t)kvh * w[5] + w[6] + hg;
   const int64_t p_step = (int64_t)w[1] * a.Hkv, s_step = (int64_t)w[5] * a.Hkv;
@@ -271,28 +280,27 @@ __global__ __launch_bounds__(256) void attn_shared_merge_kernel(SharedArgs a, in
       }
   }
   if (hq >= a.Hq) return;
-  if (lse && c == 0) lse[(int64_t)t * a.Hq + hq] = row_lse(L, M);
+  if (a.lse && c == 0) a.lse[(int64_t)t * a.Hq + hq] = row_lse(L, M);
   const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] *= inv;
-  st16(out + (int64_t)t * o_ts + (int64_t)hq * o_hs + 8 * c, pack8(acc));
+  st16(a.out + (int64_t)t * a.o_ts + (int64_t)hq * a.o_hs + 8 * c, pack8(acc));
 }
 
 template <int D>
-static void launch_shared(hipStream_t st, const SharedArgs& a, int T, int max_parts, const int32_t* tokens,
-                          uint16_t* out, int64_t o_ts, int64_t o_hs, float* lse) {
+static void launch_shared(hipStream_t st, const SharedArgs& a, int T, int max_parts, const int32_t* tokens) {
   const int items = shared_blocks(a.prefix_items, a.Hkv) + shared_blocks(a.suffix_items, a.Hkv);
   const int streams = (a.stream_items + a.B * a.splits) * (a.Hkv / a.heads);
   if (items + streams)
-    hipLaunchKernelGGL((streams ? attn_shared_kernel<D, true> : attn_shared_kernel<D, false>), dim3(items + streams),
-                       dim3(256), 0, st, a);
+    hipLaunchKernelGGL((!streams ? attn_shared_kernel<D, false, true> : a.splits ? attn_shared_kernel<D, true, false>
+                                                                            : attn_shared_kernel<D, true, true>),
+                       dim3(items + streams), dim3(256), 0, st, a);
   const int64_t units = (int64_t)T * ((a.Hq + 512 / D - 1) / (512 / D));
   if (max_parts > kNarrowParts)
-    hipLaunchKernelGGL((attn_shared_merge_kernel<D, true>), dim3((unsigned)units), dim3(256), 0, st, a, units, tokens, out,
-                       o_ts, o_hs, lse);
-  else
+    hipLaunchKernelGGL((attn_shared_merge_kernel<D, true>), dim3((unsigned)units), dim3(256), 0, st, a, units, tokens);
+  else if (max_parts)
     hipLaunchKernelGGL((attn_shared_merge_kernel<D, false>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, units,
-                       tokens, out, o_ts, o_hs, lse);
+                       tokens);
 }
 
 }  // namespace pie
@@ -310,6 +318,14 @@ enum {
 // set-up (22 requests of at most 96 tokens behind 742: 18 us, 20 with prefill items of 512; four behind 600:
 // 12.9 us, 14.2 with stream units of 256).
 constexpr int64_t kMinPrefill = 256, kMinStream = 128;
+// The longest prefix that an item of several query tokens per request walks itself, before its suffix, where no
+// suffix of the group is cut: the prefix is walked once per request instead of once per 128 rows of the group,
+// but no partial results are written and joined (213 requests of up to 19 tokens behind 143: 59 us against 81;
+// 230 behind up to 366: 55 against 66; 112 behind up to 859: 57 against 38). Head dim 256 walks a tile more
+// slowly (165 requests of up to 22 tokens behind 185: 96 us against 87; 234 behind 72: 214 against 234). Beside
+// groups that need the join all the same, only prefixes of one piece (14 requests of 2 kv heads behind up to
+// 604: 23 us with all up to 512, 17.7 with those up to 256).
+static int64_t joint_prefix(int64_t D, bool no_join) { return D == 256 ? 128 : no_join ? 512 : kMinPrefill; }
 // Query rows of a kv head that a stream unit holds.
 constexpr int64_t kStreamRows = 16;
 
@@ -376,10 +392,23 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
     return std::max<int64_t>(64, ((r.len + n - 1) / n + 63) / 64 * 64);  // whole tiles
   };
   const auto pieces = [&](const Run& r) { return r.tokens ? (r.len + piece_len(r) - 1) / piece_len(r) : 0; };
+  std::vector<char> joint((size_t)groups);  // groups whose items walk prefix and suffix
   int64_t rows, prefix_rows, items, suffix_items, stream_items, splits, max_parts, streams;
   const auto lay_out = [&] {
     rows = items = suffix_items = stream_items = splits = max_parts = 0;
-    for (const Run& r : prefix) {
+    for (bool no_join : {true, false}) {
+      bool all = true;
+      for (int64_t g = 0; g < groups; ++g) {
+        bool one = qo_indptr && prefix[(size_t)g].len <= joint_prefix(D, no_join);
+        for (int64_t b = group_indptr[g]; one && b < group_indptr[g + 1]; ++b) one = pieces(suffix[(size_t)b]) <= 1;
+        joint[(size_t)g] = one;
+        all = all && (one || prefix[(size_t)g].tokens == 0);
+      }
+      if (all) break;
+    }
+    for (int64_t g = 0; g < groups; ++g) {
+      const Run& r = prefix[(size_t)g];
+      if (joint[(size_t)g]) continue;
       rows += pieces(r) * r.tokens * Hq;
       if (r.tiles) items += pieces(r) * r.tiles;
       else stream_items += pieces(r);
@@ -388,12 +417,15 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
     prefix_rows = rows;
     if (qo_indptr) {
       int64_t most = 0;
-      for (const Run& r : suffix) {
-        const int64_t n = std::max<int64_t>(1, pieces(r));
-        rows += n * r.tokens * Hq;
-        suffix_items += n * r.tiles;
-        most = std::max(most, n);
-      }
+      for (int64_t g = 0; g < groups; ++g)
+        for (int64_t b = group_indptr[g]; b < group_indptr[g + 1]; ++b) {
+          const Run& r = suffix[(size_t)b];
+          const int64_t n = std::max<int64_t>(1, pieces(r));
+          suffix_items += n * r.tiles;
+          if (joint[(size_t)g]) continue;
+          rows += n * r.tokens * Hq;
+          most = std::max(most, n);
+        }
       max_parts += most;
     } else {
       // A decode step's suffixes grow under one plan: as many splits as 512 tokens more ask for, as long as
@@ -452,28 +484,43 @@ static int shared_plan(const int32_t* group_indptr, int64_t groups, const int32_
   PIE_REQUIRE(capacity >= words, "%s: needs %lld words, capacity %lld", what, (long long)words, (long long)capacity);
   int32_t *it = plan, *stream = plan + kItemWords * (items + suffix_items), *tok = plan + tokens_word;
   int64_t row = 0;
-  // the items of a run in order of pieces, and the part of its query tokens' words
-  const auto put = [&](const Run& r, int64_t n, int at) {
+  // the items of a run in order of pieces, and the part of its query tokens' words; pre: the prefix that a joint
+  // item walks before it
+  const auto put = [&](const Run& r, int64_t n, int at, const Run* pre) {
     const int64_t chunk = piece_len(r), run_rows = r.tokens * G;
     int32_t*& to = r.tiles ? it : stream;
     for (int64_t s = 0; s < n; ++s)
       for (int64_t r0 = 0; r0 < run_rows; r0 += kPrefillRows) {  // (a streamed run has rows of one tile at most)
         const int32_t w[kItemWords] = {(int32_t)r0, (int32_t)r.q0, (int32_t)r.tokens, (int32_t)r.len, (int32_t)r.page0,
-                                       (int32_t)(s * chunk), (int32_t)chunk, (int32_t)(row + s * Hkv * run_rows + r0)};
+                                       (int32_t)(s * chunk), (int32_t)chunk,
+                                       pre ? -1 : (int32_t)(row + s * Hkv * run_rows + r0),
+                                       pre ? (int32_t)pre->page0 : 0, pre ? (int32_t)pre->len : 0};
         memcpy(to, w, sizeof(w));
         to += kItemWords;
       }
     for (int64_t i = 0; i < r.tokens; ++i) {
-      const int32_t w[4] = {(int32_t)row, (int32_t)run_rows, (int32_t)(i * G), (int32_t)n};
+      const int32_t w[4] = {(int32_t)row, (int32_t)run_rows, (int32_t)(i * G), (int32_t)(pre ? 0 : n)};
       memcpy(tok + kTokenWords * (r.q0 + i) + at, w, sizeof(w));
     }
-    row += n * run_rows * Hkv;
+    if (!pre) row += n * run_rows * Hkv;
   };
-  for (const Run& r : prefix) put(r, pieces(r), 0);
-  for (int64_t b = 0; b < batch; ++b) {
-    if (qo_indptr) {
-      put(suffix[(size_t)b], std::max<int64_t>(1, pieces(suffix[(size_t)b])), 4);
-    } else {
+  for (int64_t g = 0; g < groups; ++g) {
+    const Run& r = prefix[(size_t)g];
+    if (!joint[(size_t)g]) {
+      put(r, pieces(r), 0, nullptr);
+      continue;
+    }
+    const int32_t w[4] = {0, 0, 0, -1};
+    for (int64_t i = 0; i < r.tokens; ++i) memcpy(tok + kTokenWords * (r.q0 + i), w, sizeof(w));
+  }
+  if (qo_indptr) {
+    for (int64_t g = 0; g < groups; ++g)
+      for (int64_t b = group_indptr[g]; b < group_indptr[g + 1]; ++b) {
+        const Run& r = suffix[(size_t)b];
+        put(r, std::max<int64_t>(1, pieces(r)), 4, joint[(size_t)g] ? &prefix[(size_t)g] : nullptr);
+      }
+  } else {
+    for (int64_t b = 0; b < batch; ++b) {
       const int32_t w[4] = {(int32_t)(row + b * splits * Hq), (int32_t)G, 0, (int32_t)-splits};
       memcpy(tok + kTokenWords * b + 4, w, sizeof(w));
     }
@@ -513,7 +560,7 @@ extern "C" int pie_hip_attention_shared(
   const int rc = paged_kv_desc(&a.kv, k_cache, v_cache, page_stride, slot_stride, head_stride, num_pages, kv_indptr,
                                kv_indices, kv_last_page_len, page_size, head_dim, what);
   if (rc) return rc;
-  PIE_REQUIRE(info && (prefix_indices || info[kInfoPrefixItems] + info[kInfoStreamItems] == 0), "%s: null argument", what);
+  PIE_REQUIRE(info && (prefix_indices || info[kInfoPrefixItems] + info[kInfoSuffixItems] + info[kInfoStreamItems] == 0), "%s: null argument", what);
   PIE_REQUIRE(info[kInfoTokens] == num_tokens && info[kInfoHq] == num_qo_heads && info[kInfoHkv] == num_kv_heads &&
                   info[kInfoDim] == head_dim && info[kInfoPage] == page_size,
               "%s: the plan is for %lld tokens, %lld/%lld heads of %lld, pages of %lld", what, (long long)info[kInfoTokens],
@@ -523,13 +570,15 @@ extern "C" int pie_hip_attention_shared(
   PIE_REQUIRE(aligned16(q) && aligned16(out) && q_tok_stride % 8 == 0 && q_head_stride % 8 == 0 && o_tok_stride % 8 == 0 &&
                   o_head_stride % 8 == 0,
               "%s: q/out pointers and strides must be 16-byte aligned", what);
-  PIE_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= info[kInfoScratch],
+  PIE_REQUIRE(info[kInfoScratch] == 0 || (scratch && aligned16(scratch) && scratch_bytes >= info[kInfoScratch]),
               "%s: needs %lld bytes of 16-byte-aligned scratch, got %lld", what, (long long)info[kInfoScratch],
               (long long)scratch_bytes);
   // a run hands its partial results from its first launch to its second
   InflightClaim claim;
-  const InflightClaim::State got = claim.take(scratch, stream);
-  if (got == InflightClaim::kBusy || got == InflightClaim::kShared) return inflight_busy(what);
+  if (info[kInfoScratch]) {
+    const InflightClaim::State got = claim.take(scratch, stream);
+    if (got == InflightClaim::kBusy || got == InflightClaim::kShared) return inflight_busy(what);
+  }
   a.q = q;
   a.q_ts = q_tok_stride;
   a.q_hs = q_head_stride;
@@ -549,14 +598,18 @@ extern "C" int pie_hip_attention_shared(
   a.part_o = static_cast<float*>(scratch);
   a.part_lse = a.part_o + info[kInfoRows] * head_dim;
   a.suffix_row = info[kInfoSuffixRow];
+  a.out = out;
+  a.o_ts = o_tok_stride;
+  a.o_hs = o_head_stride;
+  a.lse = lse;
   const int32_t* tokens = plan + info[kInfoTokensWord];
   a.order = tokens + kTokenWords * num_tokens;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int T = (int)num_tokens, parts = (int)info[kInfoMaxParts];
   switch (head_dim) {
-    case 64: launch_shared<64>(st, a, T, parts, tokens, out, o_tok_stride, o_head_stride, lse); break;
-    case 128: launch_shared<128>(st, a, T, parts, tokens, out, o_tok_stride, o_head_stride, lse); break;
-    default: launch_shared<256>(st, a, T, parts, tokens, out, o_tok_stride, o_head_stride, lse); break;
+    case 64: launch_shared<64>(st, a, T, parts, tokens); break;
+    case 128: launch_shared<128>(st, a, T, parts, tokens); break;
+    default: launch_shared<256>(st, a, T, parts, tokens); break;
   }
   return check_launch(what);
 }

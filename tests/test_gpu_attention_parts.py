@@ -340,6 +340,51 @@ def test_shared_prefix(dev, heads, sizes, prefixes, suffixes, news):
             assert (t[0] == 7).all() and (t[-1] == 7).all()
 
 
+JOINT = [  # (sizes, prefixes, suffixes, news, joined: some group's parts are joined)
+    ([3, 0, 2, 1], [500, 9, 0, 65], [40, 7, 64, 3, 1, 90], [40, 1, 33, 3, 1, 20], False),
+    ([1, 1], [64, 1], [5, 200], [9, 150], False),           # more query tokens than the suffix holds, many rows
+    ([2, 2, 1], [3000, 200, 400], [30, 2, 70, 5, 9], [13, 2, 5, 5, 9], True),
+    ([1, 2], [100, 30], [3000, 4, 8], [7, 4, 1], True),     # a suffix in pieces: its group is joined
+]
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("sizes,prefixes,suffixes,news,joined", JOINT)
+def test_short_prefixes_with_several_query_tokens(dev, heads, sizes, prefixes, suffixes, news, joined):
+    """Items that walk a prefix and their suffix and write the output, alone and beside parts that are joined; NaN in
+    the slots behind a run's last token; replays of a captured run between eager ones."""
+    for P, layout in ((16, "NHD"), (5, "HND"), (1, "NHD")):
+        print(f"short prefixes {heads} {prefixes} P={P} {layout}", flush=True)
+        c, args, kw, q, want = _shared_case(dev, sizes, prefixes, suffixes, news, heads, P, layout)
+        for ip, ix, ll in (args[1:4], args[4:7]):
+            for i, (a, b, n) in enumerate(zip(ip.tolist(), ip.tolist()[1:], ll.tolist())):
+                if b > a:
+                    page = c.data[ix[b - 1]]
+                    (page[:, n:] if layout == "NHD" else page[:, :, n:]).fill_(math.nan)
+        whole = not joined and (heads[2] != 256 or max(prefixes) <= 128)
+        w = attention.BatchSharedPrefixAttentionWrapper(_ws(dev, 64 if whole else 64 << 20), layout)
+        w.plan(*args, *heads, P, **kw)
+        assert (w._plan["info"][1] == 0) == whole
+        out = torch.full((q.shape[0] + 2, *q.shape[1:]), 7.0, dtype=BF16, device=dev)
+        lse = torch.full((q.shape[0] + 2, q.shape[1]), 7.0, device=dev)
+        w.run(q, c.arg, out=out[1:-1], lse=lse[1:-1])
+        _compare((out[1:-1], lse[1:-1]), want, "short prefixes")
+        for t in (out, lse):
+            assert (t[0] == 7).all() and (t[-1] == 7).all()
+        if P == 16:
+            eager = out.clone()
+            g = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g):
+                w.run(q, c.arg, out=out[1:-1])
+            for _ in range(3):
+                out[1:-1].zero_()
+                g.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, eager)
+                w.run(q, c.arg)
+
+
 def test_more_query_heads_per_kv_head_than_a_decode_tile(dev):
     c, args, kw, q, want = _shared_case(dev, [2], [300], [20, 9], [20, 3], (40, 2, 128), 16)
     w = attention.BatchSharedPrefixAttentionWrapper(_ws(dev))
